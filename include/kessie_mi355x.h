@@ -311,6 +311,138 @@ int kessie_rope_remap_paged(void* kv_pool, int64_t page_stride,
                             int dtype, void* stream);
 
 /* =========================================================================
+ * Rotary positions with several axes
+ * ========================================================================= */
+
+/* Rotate Q and K by positions of 1 to 4 axes (time, height, width):
+ *   ang = pos[axis(j)][t] * inv_freq[j], j < rotary_dim/2,
+ *   y1 = x1 cos - x2 sin, y2 = x1 sin + x2 cos,
+ * pairs (j, j + rotary_dim/2), or (2j, 2j+1) when `adjacent`; elements from
+ * rotary_dim on are copied.  `sections` (HOST, num_axes entries, their sum
+ * rotary_dim/2) is the number of pairs of each axis: axis 0's first, then axis
+ * 1's, ...; `interleaved` deals pair j to axis j % num_axes until that axis'
+ * section is used up, and to axis 0 from there on.  `inverse` rotates back
+ * (the gradient of the rotation).  positions: int32 (or int64 when
+ * positions_64) [num_axes][T], rows positions_axis_stride apart (0: one
+ * position for all axes).  inv_freq: fp32 [rotary_dim/2] on the device.  The
+ * product pos * inv_freq is exact, not rounded to fp32.  Element (t, h, d) of
+ * q lies at t*q_tok_stride + h*q_head_stride + d; outputs may be the inputs
+ * (in place, same strides).  q or k may be NULL (with its output).
+ * rotary_dim <= 256. */
+int kessie_rope_axes(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                     void* q_out, int64_t q_out_tok_stride,
+                     int64_t q_out_head_stride, int num_q_heads, const void* k,
+                     int64_t k_tok_stride, int64_t k_head_stride, void* k_out,
+                     int64_t k_out_tok_stride, int64_t k_out_head_stride,
+                     int num_kv_heads, const void* positions,
+                     int64_t positions_axis_stride, int positions_64,
+                     const float* inv_freq, const int32_t* sections,
+                     int num_axes, int interleaved, int adjacent, int inverse,
+                     int num_tokens, int head_dim, int rotary_dim, int dtype,
+                     void* stream);
+
+/* The same rotation on the way into the cache, in one launch: q_out receives
+ * the rotated Q (may be q; q and q_out may both be NULL), the pool the rotated
+ * K and the V of token t at slot_mapping[t] (int64; page = slot / page_size,
+ * as kessie_kv_cache_write; rows of negative slots and of pages outside
+ * [0, num_pages) are not written).  k and v themselves stay as they are. */
+int kessie_rope_axes_cache_write(
+    const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out,
+    int64_t q_out_tok_stride, int64_t q_out_head_stride, int num_q_heads,
+    const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+    int64_t v_tok_stride, int64_t v_head_stride, int num_kv_heads,
+    const void* positions, int64_t positions_axis_stride, int positions_64,
+    const float* inv_freq, const int32_t* sections, int num_axes,
+    int interleaved, int adjacent, void* kv_pool, int64_t page_stride,
+    int64_t tok_stride, int64_t kv_stride, int64_t head_stride,
+    const int64_t* slot_mapping, int page_size, int num_pages, int num_tokens,
+    int head_dim, int rotary_dim, int dtype, void* stream);
+
+/* kessie_rope_remap_paged with several axes: K of T tokens rotated in place by
+ * (tgt_pos - orig_pos)[axis(j)][t] * inv_freq[j] (the difference and the
+ * product exact).  Token t in page page_list[t / page_size]; page_list == NULL
+ * means dense rows.  No page may occur twice. */
+int kessie_rope_remap_axes(void* kv_pool, int64_t page_stride,
+                           int64_t tok_stride, int64_t head_stride,
+                           const int32_t* page_list, int num_pages,
+                           const void* orig_pos, int64_t orig_axis_stride,
+                           const void* tgt_pos, int64_t tgt_axis_stride,
+                           int positions_64, const float* inv_freq,
+                           const int32_t* sections, int num_axes,
+                           int interleaved, int adjacent, int num_tokens,
+                           int num_heads, int head_dim, int rotary_dim,
+                           int page_size, int dtype, void* stream);
+
+/* =========================================================================
+ * Cross attention
+ * ========================================================================= */
+
+/* Bytes of workspace kessie_cross_attention may need for these sizes (host
+ * call). */
+size_t kessie_cross_attention_workspace_bytes(int batch, int max_query_len,
+                                              int num_q_tokens, int num_q_heads,
+                                              int num_kv_heads, int head_dim,
+                                              int max_kv_len, int dtype);
+
+/* Attention of each sequence's queries over its own encoder states, all of
+ * them (no causal order, no window), GQA as in decode:
+ *   out = softmax(q . k^T * sm_scale) v
+ * Sequence b's queries are rows query_start_loc[b] - query_start_loc[0] ..
+ * query_start_loc[b+1] - query_start_loc[0] - 1 of q / out (int32 [batch+1],
+ * non-decreasing, at most max_query_len of them), its states rows kv_start[b]
+ * .. kv_start[b] + kv_lens[b] - 1 of k / v (int32 [batch]; at most max_kv_len;
+ * ranges may be shared, have gaps and come in any order; one that leaves
+ * [0, num_kv_tokens) is cut there).  key_mask (NULL: none): one byte a row of
+ * k / v, zero hides that state; what k and v hold there is not used, be it NaN.  A
+ * query that sees no state gives a zero row.  Rows of out past the last
+ * sequence are left as they are.  Element (t, h, d) of q at t*q_tok_stride +
+ * h*q_head_stride + d, likewise k, v and out.  head_dim <= 256; sums in fp32. */
+int kessie_cross_attention(
+    const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k,
+    int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+    int64_t v_tok_stride, int64_t v_head_stride, const int32_t* query_start_loc,
+    const int32_t* kv_start, const int32_t* kv_lens, const uint8_t* key_mask,
+    void* out, int64_t out_tok_stride, int64_t out_head_stride, int batch,
+    int max_query_len, int max_kv_len, int num_q_tokens, int num_kv_tokens,
+    int num_q_heads, int num_kv_heads, int head_dim, float sm_scale, int dtype,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* =========================================================================
+ * Tables of an engine step
+ * ========================================================================= */
+
+/* Block tables, slots and positions of a step from the requests' lengths, on
+ * the device, in one launch.  Request b holds computed_lens[b] tokens in the
+ * pages block_table[b][0 ..] (int32 rows table_stride apart, table_width
+ * entries) and brings new_lens[b] more (negative lengths count as 0).  It
+ * needs ceil((computed + new) / P) - ceil(computed / P) more pages; they are
+ * taken from free_pages (free_count[0] of at most max_free ids) in request
+ * order.  A request is granted its pages if they fit its table row, its token
+ * rows lie within num_token_rows, and it needs no page or the running sum of
+ * needs (of requests that fit their row) up to and with its own is within the
+ * free list.  Written:
+ *   block_table[b][i]   the new pages of granted requests; other entries stay
+ *   query_start_loc     int32 [batch+1], running sum of new_lens
+ *   seq_lens            int32 [batch], computed + new, or computed where not granted
+ *   slot_mapping        int64 [num_token_rows]: page * P + offset of the token; -1
+ *                       for requests not granted, pages < 0 and rows past the last token
+ *   positions           int32 [num_token_rows]: computed + index within the
+ *                       request + position_delta[b] (NULL: 0), saturating at 31
+ *                       bits; 0 past the last token
+ *   taken               int32 [1]: pages taken, the first ones of free_pages
+ *   page_valid (int8), page_positions (int32): 1 and the page's first position
+ *                       for every page taken (either may be NULL; num_pages entries). */
+int kessie_step_tables(int32_t* block_table, int64_t table_stride,
+                       int table_width, const int32_t* computed_lens,
+                       const int32_t* new_lens, const int32_t* position_delta,
+                       const int32_t* free_pages, const int32_t* free_count,
+                       int max_free, int batch, int page_size,
+                       int num_token_rows, int32_t* query_start_loc,
+                       int32_t* seq_lens, int64_t* slot_mapping,
+                       int32_t* positions, int32_t* taken, int8_t* page_valid,
+                       int32_t* page_positions, int num_pages, void* stream);
+
+/* =========================================================================
  * Paged-KV management
  * ========================================================================= */
 

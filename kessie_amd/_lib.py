@@ -72,6 +72,32 @@ SIGNATURES = {
         _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _SZ, _P]),
     # rope remap
     "kessie_rope_remap_paged": (_I, [_P, _I64, _I64, _I64, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    # rotary positions with several axes
+    # q + 2 strides, q_out + 2, Hq, k + 2, k_out + 2, Hkv, positions, axis stride, is64, inv, sections, axes,
+    # interleaved, adjacent, inverse, T, D, R, dtype, stream
+    "kessie_rope_axes": (_I, [
+        _P, _I64, _I64, _P, _I64, _I64, _I, _P, _I64, _I64, _P, _I64, _I64, _I, _P, _I64, _I, _P, _P, _I,
+        _I, _I, _I, _I, _I, _I, _I, _P]),
+    # q + 2, q_out + 2, Hq, k + 2, v + 2, Hkv, positions, axis stride, is64, inv, sections, axes, interleaved,
+    # adjacent, pool + 4 strides, slots, P, pages, T, D, R, dtype, stream
+    "kessie_rope_axes_cache_write": (_I, [
+        _P, _I64, _I64, _P, _I64, _I64, _I, _P, _I64, _I64, _P, _I64, _I64, _I, _P, _I64, _I, _P, _P, _I, _I, _I,
+        _P, _I64, _I64, _I64, _I64, _P, _I, _I, _I, _I, _I, _I, _P]),
+    # pool + 3 strides, page_list, pages, orig + stride, tgt + stride, is64, inv, sections, axes, interleaved,
+    # adjacent, T, H, D, R, P, dtype, stream
+    "kessie_rope_remap_axes": (_I, [
+        _P, _I64, _I64, _I64, _P, _I, _P, _I64, _P, _I64, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
+    # cross attention: B, max_q, T, Hq, Hkv, D, max_kv, dtype
+    "kessie_cross_attention_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    # q + 2 strides, k + 2, v + 2, q_start, kv_start, kv_lens, mask, out + 2, B, max_q, max_kv, Tq, Tkv, Hq, Hkv, D,
+    # sm_scale, dtype, ws, ws_bytes, stream
+    "kessie_cross_attention": (_I, [
+        _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64,
+        _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _SZ, _P]),
+    # table, stride, width, computed, new, delta, free, count, max_free, B, P, T, start_loc, seq_lens, slots,
+    # positions, taken, valid, page_positions, pages, stream
+    "kessie_step_tables": (_I, [
+        _P, _I64, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P]),
     # page management
     "kessie_page_insert_paged": (_I, [
         _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I, _P, _P, _P,

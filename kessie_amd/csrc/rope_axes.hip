@@ -1,0 +1,407 @@
+// Rotary positions with several axes (time, height, width), for gfx950.
+//
+//   ang_j   = pos[axis(j)][t] * inv_freq[j]          j < R/2, R <= head_dim
+//   y1, y2  = x1 cos - x2 sin, x1 sin + x2 cos       (x1, x2) = (x[j], x[j + R/2]) or, adjacent, (x[2j], x[2j+1])
+// and elements from R on as they are.  axis(j) comes from the section sizes:
+// axis 0's pairs, then axis 1's, ..., or (interleaved) dealt out in turn.
+//
+// Angles: pos * inv_freq is taken in 64 bits (exact: 31 + 24 bits), in turns,
+// and only its fraction is rounded to fp32, so a position of a million costs no
+// digits (its fp32 product is off by up to 0.03 rad).  cos and sin are
+// evaluated once per (token, pair) into LDS for all heads; the rotation is fp32
+// and rounded once.
+//
+// Three uses of one body: Q and K into tensors (or in place), Q into a tensor
+// with K and V into their cache slots, and K in place in its pages by the
+// difference of two positions.  Bound: HBM -- each row read and written once,
+// with 16-byte loads that are asked for before the angles are computed.
+#include "common.h"
+
+namespace kessie {
+namespace axes {
+namespace {
+
+constexpr int kMaxHalf = 128;  // rotary_dim <= 256
+constexpr int kMaxAxes = 4;
+
+struct Args {
+  // Rows of (token, head): x at src + t*s_ts + h*s_hs, written to dst.
+  const void* q;
+  int64_t q_ts, q_hs;
+  void* qo;
+  int64_t qo_ts, qo_hs;
+  const void* k;
+  int64_t k_ts, k_hs;
+  void* ko;
+  int64_t ko_ts, ko_hs;
+  const void* v;  // copied to the pool, never rotated
+  int64_t v_ts, v_hs;
+  // Paged destination of K (and of V, kv_stride further), by slot or by page list.
+  void* pool;
+  int64_t page_stride, tok_stride, kv_stride, head_stride;
+  const int64_t* slots;
+  const int32_t* pages;
+  int page_size, num_pages;
+  const void* pos;   // [axes][T], rows pos_as apart
+  const void* from;  // positions to take away (remap), or nullptr
+  int64_t pos_as, from_as;
+  int pos64;
+  const float* inv;
+  uint64_t axis[kMaxHalf / 32];  // two bits a pair
+  int T, Hq, Hk, Hv, D, half;
+  float sign;  // -1: rotate back
+};
+
+template <typename T>
+struct Vec16;
+template <>
+struct Vec16<bf16_t> {
+  static constexpr int N = 8;
+  typedef bf16x8 type;
+};
+template <>
+struct Vec16<f16_t> {
+  static constexpr int N = 8;
+  typedef f16x8 type;
+};
+template <>
+struct Vec16<float> {
+  static constexpr int N = 4;
+  typedef f32x4 type;
+};
+
+__device__ __forceinline__ int axis_of(const Args& a, int j) {
+  const uint64_t w = j < 64 ? (j < 32 ? a.axis[0] : a.axis[1]) : (j < 96 ? a.axis[2] : a.axis[3]);
+  return (int)(w >> (2 * (j & 31))) & 3;
+}
+
+__device__ __forceinline__ double pos_at(const void* p, int64_t i, int is64) {
+  return is64 ? (double)static_cast<const int64_t*>(p)[i] : (double)static_cast<const int32_t*>(p)[i];
+}
+
+// (cos, sin) of token t's pair j.
+__device__ __forceinline__ float2 turn(const Args& a, int t, int j) {
+  const int ax = axis_of(a, j);
+  double p = pos_at(a.pos, ax * a.pos_as + t, a.pos64);
+  if (a.from) p -= pos_at(a.from, ax * a.from_as + t, a.pos64);
+  const double r = p * (double)a.inv[j] * 0.15915494309189533577;  // turns
+  float s, c;
+  sincospif(2.0f * (float)(r - rint(r)), &s, &c);
+  return make_float2(c, s * a.sign);
+}
+
+// Element offset of token t's row in the pool, or -1: no slot, or no such page.
+__device__ __forceinline__ int64_t pool_row(const Args& a, int t) {
+  int64_t page;
+  int off;
+  if (a.slots) {
+    const int64_t slot = a.slots[t];
+    if (slot < 0) return -1;
+    page = slot / a.page_size;
+    off = (int)(slot - page * a.page_size);
+  } else {
+    const int i = t / a.page_size;
+    page = a.pages[i];
+    off = t - i * a.page_size;
+  }
+  if (page < 0 || page >= a.num_pages) return -1;
+  return page * a.page_stride + off * a.tok_stride;
+}
+
+// Where head h of token t comes from and goes to (h counts Q's, K's and V's heads); false: nowhere.
+template <typename T>
+__device__ __forceinline__ bool row_of(const Args& a, int t, int h, int64_t prow, const T*& src, T*& dst, bool& rot) {
+  rot = true;
+  if (h < a.Hq) {
+    src = static_cast<const T*>(a.q) + t * a.q_ts + h * a.q_hs;
+    dst = static_cast<T*>(a.qo) + t * a.qo_ts + h * a.qo_hs;
+    return true;
+  }
+  h -= a.Hq;
+  if (a.pool && prow < 0) return false;
+  if (h < a.Hk) {
+    dst = a.pool ? static_cast<T*>(a.pool) + prow + h * a.head_stride : static_cast<T*>(a.ko) + t * a.ko_ts + h * a.ko_hs;
+    src = a.k ? static_cast<const T*>(a.k) + t * a.k_ts + h * a.k_hs : dst;  // (no k: in place in the pages)
+    return true;
+  }
+  h -= a.Hk;
+  rot = false;
+  src = static_cast<const T*>(a.v) + t * a.v_ts + h * a.v_hs;
+  dst = static_cast<T*>(a.pool) + prow + h * a.head_stride + a.kv_stride;
+  return true;
+}
+
+// 16-byte chunks, two a thread and step: chunk pair i of a row holds both
+// halves of N pairs (or, adjacent, two neighbouring chunks), and past the
+// rotated part two chunks to copy, so every row is D / 2N steps of the same
+// kind.  kTok tokens a workgroup.
+template <typename T, bool kAdjacent, int kThreads, int kTok, int kSteps>
+__global__ __launch_bounds__(kThreads) void rope_axes_vec(Args a) {
+  typedef typename Vec16<T>::type V;
+  constexpr int N = Vec16<T>::N;
+  __shared__ float2 cs[kTok * kMaxHalf];
+  const int half = a.half, R = 2 * half;
+  const int t0 = blockIdx.x * kTok;
+  const int ntok = min(kTok, a.T - t0);
+  const int heads = a.Hq + a.Hk + a.Hv;
+  const int per = a.D / (2 * N);                 // steps a row
+  const int stride = kThreads / per;             // rows a round
+  const int i = threadIdx.x % per, r0 = threadIdx.x / per;
+  const int o1 = kAdjacent ? 2 * i * N : i * N < half ? i * N : i * N + half;
+  const int o2 = kAdjacent ? o1 + N : i * N < half ? o1 + half : o1 + (a.D - R) / 2;
+  const int rows = r0 < stride ? ntok * heads : 0;
+  bool ready = false;
+  for (int base = r0;; base += kSteps * stride) {
+    V x1[kSteps], x2[kSteps];
+    T* dst[kSteps];
+    int csi[kSteps];  // this row's angles, or -1: not rotated
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int row = base + s * stride;
+      dst[s] = nullptr;
+      csi[s] = -1;
+      if (row < rows) {
+        const int tt = kTok == 1 ? 0 : kTok == 2 ? (row >= heads ? 1 : 0) : row / heads;
+        const int h = row - tt * heads;
+        const T* src;
+        T* to;
+        bool rot;
+        if (row_of<T>(a, t0 + tt, h, a.pool && h >= a.Hq ? pool_row(a, t0 + tt) : 0, src, to, rot)) {
+          if (rot) csi[s] = tt * half;
+          if (src != to || o1 < R) {  // (in place, the rest of the row stays)
+            dst[s] = to;
+            x1[s] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src + o1));
+            x2[s] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src + o2));
+          }
+        }
+      }
+    }
+    if (!ready) {
+      for (int n = threadIdx.x; n < ntok * half; n += kThreads) {
+        const int tt = n / half;
+        cs[n] = turn(a, t0 + tt, n - tt * half);
+      }
+      __syncthreads();
+      ready = true;
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      if (dst[s] == nullptr) continue;
+      V y1 = x1[s], y2 = x2[s];
+      if (csi[s] >= 0) {
+        if constexpr (kAdjacent) {
+          // (rotary_dim is a multiple of N: a chunk is rotated whole or not at all)
+          auto rotate = [&](V x, int o) {
+            if (o >= R) return x;
+            V y;
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+              const float2 w = cs[csi[s] + ((o + e) >> 1)];
+              const float u = to_f32(x[e]), z = to_f32(x[e + 1]);
+              y[e] = from_f32<T>(fmaf(u, w.x, -(z * w.y)));
+              y[e + 1] = from_f32<T>(fmaf(u, w.y, z * w.x));
+            }
+            return y;
+          };
+          y1 = rotate(x1[s], o1);
+          y2 = rotate(x2[s], o2);
+        } else if (o1 < half) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float2 w = cs[csi[s] + o1 + e];
+            const float u = to_f32(x1[s][e]), z = to_f32(x2[s][e]);
+            y1[e] = from_f32<T>(fmaf(u, w.x, -(z * w.y)));
+            y2[e] = from_f32<T>(fmaf(u, w.y, z * w.x));
+          }
+        }
+      }
+      __builtin_nontemporal_store(y1, reinterpret_cast<V*>(dst[s] + o1));
+      __builtin_nontemporal_store(y2, reinterpret_cast<V*>(dst[s] + o2));
+    }
+    if (base - r0 + kSteps * stride >= ntok * heads) break;  // (uniform)
+  }
+}
+
+// Any head_dim and alignment: one thread a pair, or a copied element pair.
+template <typename T, bool kAdjacent>
+__global__ __launch_bounds__(256) void rope_axes_scalar(Args a) {
+  const int heads = a.Hq + a.Hk + a.Hv;
+  const int R = 2 * a.half, per = a.half + (a.D - R);  // pairs, then single elements
+  const int64_t total = (int64_t)a.T * heads * per;
+  for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < total; n += (int64_t)gridDim.x * 256) {
+    const int i = (int)(n % per);
+    const int64_t th = n / per;
+    const int t = (int)(th / heads), h = (int)(th - (int64_t)t * heads);
+    const T* src;
+    T* dst;
+    bool rot;
+    if (!row_of<T>(a, t, h, a.pool && h >= a.Hq ? pool_row(a, t) : 0, src, dst, rot)) continue;
+    if (i >= a.half) {
+      const int d = R + i - a.half;
+      if (src != dst) dst[d] = src[d];
+      continue;
+    }
+    const int d1 = kAdjacent ? 2 * i : i, d2 = kAdjacent ? 2 * i + 1 : i + a.half;
+    if (!rot) {
+      dst[d1] = src[d1];
+      dst[d2] = src[d2];
+      continue;
+    }
+    const float2 w = turn(a, t, i);
+    const float u = to_f32(src[d1]), z = to_f32(src[d2]);
+    dst[d1] = from_f32<T>(fmaf(u, w.x, -(z * w.y)));
+    dst[d2] = from_f32<T>(fmaf(u, w.y, z * w.x));
+  }
+}
+
+template <typename T, bool kAdjacent>
+int launch(const Args& a, hipStream_t s) {
+  constexpr int N = Vec16<T>::N;
+  const int R = 2 * a.half, per = a.D / (2 * N);
+  auto fine = [](const void* p, int64_t s1, int64_t s2) { return p == nullptr || (aligned16(p) && s1 % N == 0 && s2 % N == 0); };
+  const bool vec = a.D % (2 * N) == 0 && per <= 64 && (kAdjacent ? R % N == 0 : a.half % N == 0 && (a.D - R) % (2 * N) == 0) &&
+                   fine(a.q, a.q_ts, a.q_hs) && fine(a.qo, a.qo_ts, a.qo_hs) && fine(a.k, a.k_ts, a.k_hs) &&
+                   fine(a.ko, a.ko_ts, a.ko_hs) && fine(a.v, a.v_ts, a.v_hs) && fine(a.pool, a.tok_stride, a.head_stride) &&
+                   (a.pool == nullptr || (a.page_stride % N == 0 && a.kv_stride % N == 0));
+  const int heads = a.Hq + a.Hk + a.Hv;
+  if (!vec) {
+    const int64_t items = (int64_t)a.T * heads * (a.half + a.D - R);
+    const int64_t grid = (items + 255) / 256;
+    hipLaunchKernelGGL((rope_axes_scalar<T, kAdjacent>), dim3((unsigned)(grid < (1 << 20) ? grid : 1 << 20)), dim3(256), 0, s, a);
+  } else if (a.k == nullptr && a.Hq == 0) {  // in place in the pages
+    hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, 1024, 16, 1>), dim3(div_up(a.T, 16)), dim3(1024), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, 256, 2, 3>), dim3(div_up(a.T, 2)), dim3(256), 0, s, a);
+  }
+  return check_launch("rope axes");
+}
+
+// Checks what the three entries share, fills the axis map and launches.
+int dispatch(Args& a, const int32_t* sections, int num_axes, int interleaved, int adjacent, int inverse, int rotary_dim,
+             int dtype, hipStream_t s) {
+  KESSIE_REQUIRE(a.T >= 0 && a.D > 0 && a.Hq >= 0 && a.Hk >= 0, KESSIE_ERR_INVALID, "rope axes: bad sizes T=%d Hq=%d Hkv=%d D=%d",
+                 a.T, a.Hq, a.Hk, a.D);
+  KESSIE_REQUIRE(rotary_dim > 0 && rotary_dim % 2 == 0 && rotary_dim <= a.D, KESSIE_ERR_INVALID,
+                 "rope axes: rotary_dim %d (even, at most head_dim %d)", rotary_dim, a.D);
+  a.half = rotary_dim / 2;
+  KESSIE_REQUIRE(a.half <= kMaxHalf, KESSIE_ERR_UNSUPPORTED, "rope axes: rotary_dim %d above %d", rotary_dim, 2 * kMaxHalf);
+  KESSIE_REQUIRE(sections != nullptr && num_axes >= 1 && num_axes <= kMaxAxes, KESSIE_ERR_INVALID, "rope axes: %d axes (1 to %d)",
+                 num_axes, kMaxAxes);
+  int64_t sum = 0;
+  for (int i = 0; i < num_axes; ++i) {
+    KESSIE_REQUIRE(sections[i] >= 0, KESSIE_ERR_INVALID, "rope axes: section %d has %d pairs", i, sections[i]);
+    sum += sections[i];
+  }
+  KESSIE_REQUIRE(sum == a.half, KESSIE_ERR_INVALID, "rope axes: sections hold %lld pairs, rotary_dim %d has %d", (long long)sum,
+                 rotary_dim, a.half);
+  for (auto& w : a.axis) w = 0;
+  int left[kMaxAxes] = {};
+  for (int i = 0; i < num_axes; ++i) left[i] = sections[i];
+  for (int j = 0, ax = 0; j < a.half; ++j) {
+    int use = ax;
+    if (interleaved) {
+      // Pair j is axis j mod A's until that section is used up, and axis 0's after.
+      use = j % num_axes;
+      if (j >= num_axes * sections[use]) use = 0;
+    } else {
+      while (left[ax] == 0) ++ax;
+      use = ax;
+    }
+    KESSIE_REQUIRE(left[use] > 0, KESSIE_ERR_INVALID,
+                   "rope axes: interleaved sections must leave the surplus to axis 0 (axis %d gets more pairs than its section)", use);
+    --left[use];
+    a.axis[j >> 5] |= (uint64_t)use << (2 * (j & 31));
+  }
+  a.sign = inverse ? -1.0f : 1.0f;
+  if (a.T == 0 || a.Hq + a.Hk == 0) return KESSIE_OK;
+  KESSIE_REQUIRE(a.pos && a.inv, KESSIE_ERR_INVALID, "rope axes: null pointer");
+  switch (dtype) {
+    case KESSIE_DTYPE_BF16: return adjacent ? launch<bf16_t, true>(a, s) : launch<bf16_t, false>(a, s);
+    case KESSIE_DTYPE_F16: return adjacent ? launch<f16_t, true>(a, s) : launch<f16_t, false>(a, s);
+    case KESSIE_DTYPE_F32: return adjacent ? launch<float, true>(a, s) : launch<float, false>(a, s);
+  }
+  set_error(KESSIE_ERR_UNSUPPORTED, "rope axes: dtype %d", dtype);
+  return KESSIE_ERR_UNSUPPORTED;
+}
+
+}  // namespace
+}  // namespace axes
+}  // namespace kessie
+
+using namespace kessie;
+using namespace kessie::axes;
+
+extern "C" int kessie_rope_axes(const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out,
+                                int64_t q_out_tok_stride, int64_t q_out_head_stride, int num_q_heads, const void* k,
+                                int64_t k_tok_stride, int64_t k_head_stride, void* k_out, int64_t k_out_tok_stride,
+                                int64_t k_out_head_stride, int num_kv_heads, const void* positions,
+                                int64_t positions_axis_stride, int positions_64, const float* inv_freq,
+                                const int32_t* sections, int num_axes, int interleaved, int adjacent, int inverse,
+                                int num_tokens, int head_dim, int rotary_dim, int dtype, void* stream) {
+  clear_error();
+  Args a{};
+  a.q = q, a.q_ts = q_tok_stride, a.q_hs = q_head_stride;
+  a.qo = q_out, a.qo_ts = q_out_tok_stride, a.qo_hs = q_out_head_stride;
+  a.k = k, a.k_ts = k_tok_stride, a.k_hs = k_head_stride;
+  a.ko = k_out, a.ko_ts = k_out_tok_stride, a.ko_hs = k_out_head_stride;
+  a.pos = positions, a.pos_as = positions_axis_stride, a.pos64 = positions_64;
+  a.inv = inv_freq;
+  a.T = num_tokens, a.Hq = q ? num_q_heads : 0, a.Hk = k ? num_kv_heads : 0, a.D = head_dim;
+  KESSIE_REQUIRE((q == nullptr) == (q_out == nullptr) && (k == nullptr) == (k_out == nullptr), KESSIE_ERR_INVALID,
+                 "rope axes: an input without its output");
+  return dispatch(a, sections, num_axes, interleaved, adjacent, inverse, rotary_dim, dtype, as_stream(stream));
+}
+
+extern "C" int kessie_rope_axes_cache_write(
+    const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out, int64_t q_out_tok_stride,
+    int64_t q_out_head_stride, int num_q_heads, const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+    int64_t v_tok_stride, int64_t v_head_stride, int num_kv_heads, const void* positions, int64_t positions_axis_stride,
+    int positions_64, const float* inv_freq, const int32_t* sections, int num_axes, int interleaved, int adjacent,
+    void* kv_pool, int64_t page_stride, int64_t tok_stride, int64_t kv_stride, int64_t head_stride,
+    const int64_t* slot_mapping, int page_size, int num_pages, int num_tokens, int head_dim, int rotary_dim, int dtype,
+    void* stream) {
+  clear_error();
+  Args a{};
+  a.q = q, a.q_ts = q_tok_stride, a.q_hs = q_head_stride;
+  a.qo = q_out, a.qo_ts = q_out_tok_stride, a.qo_hs = q_out_head_stride;
+  a.k = k, a.k_ts = k_tok_stride, a.k_hs = k_head_stride;
+  a.v = v, a.v_ts = v_tok_stride, a.v_hs = v_head_stride;
+  a.pool = kv_pool, a.page_stride = page_stride, a.tok_stride = tok_stride, a.kv_stride = kv_stride, a.head_stride = head_stride;
+  a.slots = slot_mapping, a.page_size = page_size, a.num_pages = num_pages;
+  a.pos = positions, a.pos_as = positions_axis_stride, a.pos64 = positions_64;
+  a.inv = inv_freq;
+  a.T = num_tokens, a.Hq = q ? num_q_heads : 0, a.Hk = num_kv_heads, a.Hv = num_kv_heads, a.D = head_dim;
+  KESSIE_REQUIRE((q == nullptr) == (q_out == nullptr), KESSIE_ERR_INVALID, "rope axes: an input without its output");
+  KESSIE_REQUIRE(page_size > 0 && num_pages >= 0 && num_kv_heads > 0, KESSIE_ERR_INVALID, "rope axes: bad sizes P=%d pages=%d Hkv=%d",
+                 page_size, num_pages, num_kv_heads);
+  KESSIE_REQUIRE(num_tokens <= 0 || (k && v && kv_pool && slot_mapping), KESSIE_ERR_INVALID, "rope axes: null pointer");
+  KESSIE_REQUIRE(head_stride >= head_dim && tok_stride >= (int64_t)num_kv_heads * head_stride && kv_stride > 0, KESSIE_ERR_INVALID,
+                 "rope axes: pool strides overlap");
+  return dispatch(a, sections, num_axes, interleaved, adjacent, 0, rotary_dim, dtype, as_stream(stream));
+}
+
+extern "C" int kessie_rope_remap_axes(void* kv_pool, int64_t page_stride, int64_t tok_stride, int64_t head_stride,
+                                      const int32_t* page_list, int num_pages, const void* orig_pos,
+                                      int64_t orig_axis_stride, const void* tgt_pos, int64_t tgt_axis_stride,
+                                      int positions_64, const float* inv_freq, const int32_t* sections, int num_axes,
+                                      int interleaved, int adjacent, int num_tokens, int num_heads, int head_dim,
+                                      int rotary_dim, int page_size, int dtype, void* stream) {
+  clear_error();
+  Args a{};
+  a.pos = tgt_pos, a.pos_as = tgt_axis_stride, a.pos64 = positions_64;
+  a.from = orig_pos, a.from_as = orig_axis_stride;
+  a.inv = inv_freq;
+  a.T = num_tokens, a.Hk = num_heads, a.D = head_dim;
+  KESSIE_REQUIRE(num_heads > 0 && head_stride >= head_dim && tok_stride >= (int64_t)num_heads * head_stride, KESSIE_ERR_INVALID,
+                 "rope axes: strides overlap (tok %lld head %lld)", (long long)tok_stride, (long long)head_stride);
+  KESSIE_REQUIRE(num_tokens <= 0 || (kv_pool && orig_pos), KESSIE_ERR_INVALID, "rope axes: null pointer");
+  if (page_list) {
+    KESSIE_REQUIRE(page_size > 0 && num_pages >= 0, KESSIE_ERR_INVALID, "rope axes: page_size=%d num_pages=%d", page_size, num_pages);
+    a.pool = kv_pool, a.page_stride = page_stride, a.tok_stride = tok_stride, a.head_stride = head_stride;
+    a.pages = page_list, a.page_size = page_size, a.num_pages = num_pages;
+  } else {  // dense rows
+    a.k = a.ko = kv_pool;
+    a.k_ts = a.ko_ts = tok_stride, a.k_hs = a.ko_hs = head_stride;
+  }
+  return dispatch(a, sections, num_axes, interleaved, adjacent, 0, rotary_dim, dtype, as_stream(stream));
+}

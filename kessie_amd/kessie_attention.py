@@ -32,7 +32,7 @@ import logging
 import os
 import threading
 from dataclasses import dataclass
-from typing import Optional, Set
+from typing import Optional, Sequence, Set
 
 import torch
 
@@ -317,6 +317,64 @@ class KeSSieAttentionMetadata:
     slot_mapping: torch.Tensor
     query_start_loc_cpu: Optional[torch.Tensor] = None
     seq_lens_cpu: Optional[torch.Tensor] = None
+    # What build() adds: the token rows' positions (int32, device) and the
+    # number of pages it took from the front of the free list.
+    positions: Optional[torch.Tensor] = None
+    pages_taken: int = 0
+
+    @classmethod
+    def build(cls, block_table: torch.Tensor, computed_lens: Sequence[int], new_lens: Sequence[int], page_size: int,
+              free_pages: Optional[torch.Tensor] = None, num_free: Optional[int] = None,
+              num_token_rows: Optional[int] = None, position_delta: Optional[Sequence[int]] = None,
+              page_valid: Optional[torch.Tensor] = None, page_positions: Optional[torch.Tensor] = None
+              ) -> "KeSSieAttentionMetadata":
+        """The metadata of one engine step from its requests' lengths (host
+        sequences): one small copy to the device and one launch
+        (ops.step_tables) give the new pages' table entries (block_table int32
+        [B, W], in place), slots, positions and offsets.  free_pages int32 on
+        the device, its first num_free entries (default: all) free; the pages
+        taken are its first ``pages_taken``.  num_token_rows pads slot_mapping
+        and positions (a captured graph's size).  Raises ValueError, having
+        changed nothing, when the pages, the table's rows or the token rows do
+        not suffice."""
+        from . import ops
+
+        have, new = [int(x) for x in computed_lens], [int(x) for x in new_lens]
+        delta = [0] * len(have) if position_delta is None else [int(x) for x in position_delta]
+        if len(new) != len(have) or len(delta) != len(have):
+            raise ValueError("computed_lens, new_lens and position_delta differ in length")
+        if any(x < 0 for x in have) or any(x < 0 for x in new):
+            raise ValueError("negative lengths")
+        if page_size <= 0:
+            raise ValueError(f"page_size {page_size}")
+        if block_table.dim() != 2 or block_table.shape[0] < len(have):
+            raise ValueError(f"block_table must be [B, W] with {len(have)} rows or more, got {tuple(block_table.shape)}")
+        total = [c + n for c, n in zip(have, new)]
+        need = sum(-(-s // page_size) - -(-c // page_size) for c, s in zip(have, total))
+        free = 0 if free_pages is None else free_pages.numel() if num_free is None else min(int(num_free), free_pages.numel())
+        tokens = sum(new)
+        rows = tokens if num_token_rows is None else int(num_token_rows)
+        if need > free:
+            raise ValueError(f"the step needs {need} pages, {free} are free")
+        if total and -(-max(total) // page_size) > block_table.shape[1]:
+            raise ValueError(f"a request of {max(total)} tokens exceeds the block table's {block_table.shape[1]} pages")
+        if tokens > rows:
+            raise ValueError(f"{tokens} tokens exceed {rows} token rows")
+        b, dev = len(have), block_table.device
+        host = torch.tensor([*have, *new, *delta, free], dtype=torch.int32)
+        if dev.type == "cuda":
+            host = host.pin_memory()
+        sent = host.to(dev, non_blocking=True)
+        t = ops.step_tables(block_table, sent[:b], sent[b:2 * b], page_size, rows, free_pages,
+                            None if free_pages is None else sent[3 * b:], position_delta=sent[2 * b:3 * b],
+                            page_valid=page_valid, page_positions=page_positions)
+        starts = [0]
+        for n in new:
+            starts.append(starts[-1] + n)
+        return cls(num_actual_tokens=tokens, max_query_len=max(new, default=0), query_start_loc=t.query_start_loc,
+                   max_seq_len=max(total, default=0), seq_lens=t.seq_lens, block_table=block_table[:b],
+                   slot_mapping=t.slot_mapping, query_start_loc_cpu=torch.tensor(starts, dtype=torch.int32),
+                   seq_lens_cpu=torch.tensor(total, dtype=torch.int32), positions=t.positions, pages_taken=need)
 
 
 class KeSSieAttentionBackend(AttentionBackend):

@@ -15,7 +15,8 @@ Differences a caller can observe:
     kessie_kernels_v2.hip:592); results follow kessie_hip_kernels.py:592-593.
   * failures raise ``KeSSieError`` instead of printing to stderr.
 Added: the paged entry points (fog decode / prefill, paged RoPE remap, page
-insert / select-evict / compact / gather / valid list / evict list).
+insert / select-evict / compact / gather / valid list / evict list), the RoPE
+remap with several position axes and cross attention.
 """
 from __future__ import annotations
 
@@ -178,6 +179,22 @@ class KeSSieKernels:
                              rope_theta, page_list=page_list.to(torch.int32), layout=layout,
                              stream=self._resolve_stream(stream))
         self._finish(stream)
+
+    def rope_remap_axes(self, pool, page_list, orig_positions, target_positions, inv_freq, sections,
+                        interleaved: bool = False, adjacent: bool = False, layout: str = "native", stream=None):
+        """Positions [axes, T]; page_list None: pool is a dense K tensor [T, H, D]."""
+        ops.rope_remap_axes(pool, orig_positions, target_positions, inv_freq, sections, interleaved, adjacent,
+                            page_list=None if page_list is None else page_list.to(torch.int32), layout=layout,
+                            stream=self._resolve_stream(stream))
+        self._finish(stream)
+
+    def cross_attention(self, q, k, v, query_start_loc, max_query_len: int, kv_start, kv_lens, max_kv_len: int,
+                        key_mask=None, sm_scale=None, stream=None):
+        """q [T, Hq, D] over each sequence's own rows of k, v [N, Hkv, D]."""
+        out = ops.cross_attention(q, k, v, query_start_loc, max_query_len, kv_start, kv_lens, max_kv_len,
+                                  key_mask=key_mask, sm_scale=sm_scale, stream=self._resolve_stream(stream))
+        self._finish(stream)
+        return out
 
     def page_select_evict(self, scores, page_valid, k_evict: int = -1, evict_fraction: float = 0.25,
                           stream=None):

@@ -12,11 +12,12 @@ Pool layouts (the innermost head_dim axis must be contiguous):
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 import threading
 from dataclasses import dataclass
-from typing import Optional
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
@@ -428,6 +429,341 @@ def rope_remap_paged(pool: torch.Tensor, orig_pos: torch.Tensor, tgt_pos: torch.
     _lib.check("kessie_rope_remap_paged", lib.kessie_rope_remap_paged(
         ptr, ps, ts, hs, _ptr(page_list), n_pages, _ptr(_contig(orig_pos, "orig_pos")),
         _ptr(_contig(tgt_pos, "tgt_pos")), _ptr(inv), t, h, d, p_size, dt, _stream_ptr(stream, device)))
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions with several axes
+# ---------------------------------------------------------------------------
+def _one_device(dev: torch.device, **tensors: Optional[torch.Tensor]) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, not on {dev}")
+
+
+_here = contextlib.nullcontext()
+
+
+def _on(dev: torch.device):
+    """The device a launch belongs to made current (nothing to do where it is already)."""
+    return _here if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+_sections: dict = {}
+
+
+def _sections_arg(sections: Sequence[int]):
+    key = tuple(sections)
+    got = _sections.get(key)
+    if got is None:
+        if not 1 <= len(key) <= 4:
+            raise ValueError(f"sections must name 1 to 4 axes, got {len(key)}")
+        got = _sections[key] = (C.c_int32 * len(key))(*key)
+    return got
+
+
+def _positions_arg(p: torch.Tensor, axes: int, t: int, name: str) -> int:
+    """The stride between the axes' rows of positions [axes, T], or 0 for [T]."""
+    if p.dtype != torch.int32 and p.dtype != torch.int64:
+        raise TypeError(f"{name} must be int32 or int64")
+    if p.dim() == 1 and p.shape[0] == t:
+        step, row = p.stride(0), 0
+    elif p.dim() == 2 and p.shape[0] == axes and p.shape[1] == t:
+        step, row = p.stride(1), p.stride(0)
+    else:
+        raise ValueError(f"{name} must be [{t}] or [{axes}, {t}], got {tuple(p.shape)}")
+    if step != 1 and t > 1:
+        raise ValueError(f"{name} must be contiguous along the tokens")
+    return row
+
+
+def _inv_arg(inv_freq: torch.Tensor, d: int) -> int:
+    """rotary_dim of a frequency table."""
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous float32 vector")
+    r = 2 * inv_freq.shape[0]
+    if r > d:
+        raise ValueError(f"inv_freq has {r // 2} entries, more than half of head_dim {d}")
+    return r
+
+
+def _rows3(x: torch.Tensor, name: str, shape=None, dtype=None) -> None:
+    if x.dim() != 3 or (shape is not None and tuple(x.shape) != tuple(shape)):
+        raise ValueError(f"{name} must be {'[T, H, D]' if shape is None else tuple(shape)}, got {tuple(x.shape)}")
+    if dtype is not None and x.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {x.dtype}")
+    if x.stride(2) != 1:
+        raise ValueError(f"{name} head_dim axis must be contiguous")
+
+
+def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
+              sections: Sequence[int], interleaved: bool = False, adjacent: bool = False, inverse: bool = False,
+              q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None, stream=None):
+    """Rotate q [T, Hq, D] and k [T, Hkv, D] (or None; any token/head strides)
+    by positions with several axes, in place unless q_out / k_out are given.
+    Returns (q_out, k_out).
+
+    positions int32 or int64 [A, T], or [T] for one position on all axes;
+    inv_freq fp32 [R/2] (``inv_freq_table(R, theta, device)``), R <= D elements
+    of a head being rotated; ``sections`` the pairs of each axis, axis 0's
+    first, or (``interleaved``) dealt out in turn with the surplus on axis 0;
+    pairs are (j, j + R/2), or neighbours when ``adjacent``.  ``inverse``
+    rotates back, which is the gradient of the rotation too."""
+    _rows3(q, "q")
+    t, hq, d = q.shape
+    if q_out is None:
+        q_out = q
+    else:
+        _rows3(q_out, "q_out", q.shape, q.dtype)
+    hkv = ks0 = ks1 = os0 = os1 = 0
+    if k is not None:
+        _rows3(k, "k", (t, k.shape[1], d), q.dtype)
+        if k_out is None:
+            k_out = k
+        else:
+            _rows3(k_out, "k_out", k.shape, k.dtype)
+        hkv, (ks0, ks1, _), (os0, os1, _) = k.shape[1], k.stride(), k_out.stride()
+    elif k_out is not None:
+        raise ValueError("k_out without k")
+    row = _positions_arg(positions, len(sections), t, "positions")
+    r = _inv_arg(inv_freq, d)
+    dev = q.device
+    _one_device(dev, k=k, q_out=q_out, k_out=k_out, positions=positions, inv_freq=inv_freq)
+    with _on(dev):
+        _lib.check("kessie_rope_axes", _lib.load().kessie_rope_axes(
+            _ptr(q), q.stride(0), q.stride(1), _ptr(q_out), q_out.stride(0), q_out.stride(1), hq, _ptr(k), ks0, ks1,
+            _ptr(k_out), os0, os1, hkv, _ptr(positions), row, positions.dtype == torch.int64, _ptr(inv_freq),
+            _sections_arg(sections), len(sections), interleaved, adjacent, inverse, t, d, r, dtype_code(q.dtype),
+            _stream_ptr(stream, dev)))
+    return q_out, k_out
+
+
+def rope_axes_cache_write(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                          pool: torch.Tensor, slot_mapping: torch.Tensor, inv_freq: torch.Tensor,
+                          sections: Sequence[int], interleaved: bool = False, adjacent: bool = False,
+                          q_out: Optional[torch.Tensor] = None, layout: str = "native", stream=None):
+    """``rope_axes`` and ``kv_cache_write`` in one launch: q (or None) rotated
+    in place or into q_out, rotated k and v [T, Hkv, D] written to the paged
+    pool at slot_mapping[t] (int64, negative: not written).  k and v stay as
+    they are.  Returns q_out."""
+    pv = pool_view(pool, layout)
+    _rows3(k, "k")
+    t, h, d = k.shape
+    if h != pv.num_kv_heads or d != pv.head_dim:
+        raise ValueError("k/v heads or head_dim do not match the pool")
+    if k.dtype != pool.dtype:
+        raise TypeError("k/v dtype must match the pool")
+    _rows3(v, "v", k.shape, k.dtype)
+    hq = qs0 = qs1 = os0 = os1 = 0
+    if q is not None:
+        _rows3(q, "q", (t, q.shape[1], d), k.dtype)
+        if q_out is None:
+            q_out = q
+        else:
+            _rows3(q_out, "q_out", q.shape, q.dtype)
+        hq, (qs0, qs1, _), (os0, os1, _) = q.shape[1], q.stride(), q_out.stride()
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() < t:
+        raise ValueError("slot_mapping must be int64 with one entry per token")
+    row = _positions_arg(positions, len(sections), t, "positions")
+    r = _inv_arg(inv_freq, d)
+    dev = pool.device
+    _one_device(dev, q=q, q_out=q_out, k=k, v=v, positions=positions, slot_mapping=slot_mapping, inv_freq=inv_freq)
+    with _on(dev):
+        _lib.check("kessie_rope_axes_cache_write", _lib.load().kessie_rope_axes_cache_write(
+            _ptr(q), qs0, qs1, _ptr(q_out), os0, os1, hq, _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0),
+            v.stride(1), h, _ptr(positions), row, positions.dtype == torch.int64, _ptr(inv_freq),
+            _sections_arg(sections), len(sections), interleaved, adjacent, C.c_void_p(pv.k_ptr), pv.page_stride,
+            pv.tok_stride, pv.kv_stride, pv.head_stride, _ptr(_contig(slot_mapping, "slot_mapping")), pv.page_size,
+            pv.num_pages, t, d, r, dtype_code(k.dtype), _stream_ptr(stream, dev)))
+    return q_out
+
+
+def rope_remap_axes(pool: torch.Tensor, orig_pos: torch.Tensor, tgt_pos: torch.Tensor, inv_freq: torch.Tensor,
+                    sections: Sequence[int], interleaved: bool = False, adjacent: bool = False,
+                    page_list: Optional[torch.Tensor] = None, layout: str = "native", stream=None) -> None:
+    """``rope_remap_paged`` with several axes: recalled K of T tokens re-rotated
+    in place from orig_pos to tgt_pos (int32 or int64, [A, T] or [T]), token t
+    in page page_list[t // P], slot t % P (no page twice).  With page_list None,
+    ``pool`` is a dense K tensor [T, H, D] (any token/head strides)."""
+    axes = len(sections)
+    t = orig_pos.shape[-1]
+    if orig_pos.dtype != tgt_pos.dtype:
+        raise TypeError("orig_pos and tgt_pos must have one dtype")
+    r0 = _positions_arg(orig_pos, axes, t, "orig_pos")
+    r1 = _positions_arg(tgt_pos, axes, t, "tgt_pos")
+    if page_list is None:
+        _rows3(pool, "k", (t,) + tuple(pool.shape[1:]))
+        _, h, d = pool.shape
+        ptr, ps, (ts, hs, _), n_pages, p_size = _ptr(pool), 0, pool.stride(), 0, 0
+    else:
+        pv = pool_view(pool, layout)
+        if page_list.dtype != torch.int32 or not page_list.is_contiguous():
+            raise TypeError("page_list must be contiguous int32")
+        if page_list.numel() * pv.page_size < t:
+            raise ValueError("page_list too short for the token count")
+        ptr, ps, ts, hs = C.c_void_p(pv.k_ptr), pv.page_stride, pv.tok_stride, pv.head_stride
+        n_pages, p_size, h, d = pv.num_pages, pv.page_size, pv.num_kv_heads, pv.head_dim
+    r = _inv_arg(inv_freq, d)
+    dev = pool.device
+    _one_device(dev, orig_pos=orig_pos, tgt_pos=tgt_pos, inv_freq=inv_freq, page_list=page_list)
+    with _on(dev):
+        _lib.check("kessie_rope_remap_axes", _lib.load().kessie_rope_remap_axes(
+            ptr, ps, ts, hs, _ptr(page_list), n_pages, _ptr(orig_pos), r0, _ptr(tgt_pos), r1,
+            orig_pos.dtype == torch.int64, _ptr(inv_freq), _sections_arg(sections), axes, interleaved, adjacent, t, h, d,
+            r, p_size, dtype_code(pool.dtype), _stream_ptr(stream, dev)))
+
+
+# ---------------------------------------------------------------------------
+# Cross attention
+# ---------------------------------------------------------------------------
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_start_loc: torch.Tensor,
+                    max_query_len: int, kv_start: torch.Tensor, kv_lens: torch.Tensor, max_kv_len: int,
+                    key_mask: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None, ws: Optional[torch.Tensor] = None,
+                    stream=None) -> torch.Tensor:
+    """Attention of B sequences' queries over their own encoder states, without
+    causal order: q [T, Hq, D] packed, sequence b's queries at rows
+    query_start_loc[b] - query_start_loc[0] .. (int32 [B+1]), its states at
+    rows kv_start[b] .. kv_start[b] + kv_lens[b] - 1 (int32 [B]) of k and v
+    [N, Hkv, D] (any token/head strides, so slices of one projection, or a
+    padded [B, L, Hkv, D] viewed as [B*L, Hkv, D]).  Several rows that read the
+    same states (beams) are best one sequence.
+
+    ``max_query_len`` and ``max_kv_len`` are host-side upper bounds (longer
+    sequences are cut there); key_mask (bool or uint8 [N]) hides states where
+    it is zero.  A query without states gives zeros; rows of out behind the
+    last sequence are left as they were.  ws: workspace for split partials (a
+    cached one when None)."""
+    _rows3(q, "q")
+    t, hq, d = q.shape
+    _rows3(k, "k", (k.shape[0], k.shape[1], d), q.dtype)
+    n, hkv, _ = k.shape
+    _rows3(v, "v", k.shape, q.dtype)
+    if hq % hkv:
+        raise ValueError(f"{hq} query heads are no multiple of {hkv} kv heads")
+    b = kv_lens.numel()
+    if query_start_loc.dtype != torch.int32 or kv_start.dtype != torch.int32 or kv_lens.dtype != torch.int32:
+        raise TypeError("query_start_loc, kv_start and kv_lens must be int32")
+    if query_start_loc.numel() != b + 1 or kv_start.numel() != b:
+        raise ValueError("query_start_loc must hold B+1 entries, kv_start and kv_lens B")
+    if max_query_len < 0 or max_kv_len < 0:
+        raise ValueError("max_query_len and max_kv_len must not be negative")
+    if max(t, n) >= 1 << 31:
+        raise ValueError(f"{t} queries, {n} states: fewer than 2^31 are taken")
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool and key_mask.dtype != torch.uint8:
+            raise TypeError("key_mask must be bool or uint8")
+        if key_mask.dim() != 1 or key_mask.shape[0] != n:
+            raise ValueError(f"key_mask must be [{n}], got {tuple(key_mask.shape)}")
+        _contig(key_mask, "key_mask")
+    if out is None:
+        out = torch.empty(t, hq, d, dtype=q.dtype, device=q.device)
+    else:
+        _rows3(out, "out", q.shape, q.dtype)
+    dev = q.device
+    _one_device(dev, k=k, v=v, query_start_loc=query_start_loc, kv_start=kv_start, kv_lens=kv_lens, key_mask=key_mask,
+                out=out, ws=ws)
+    dt = dtype_code(q.dtype)
+    mq, mk = min(int(max_query_len), t), min(int(max_kv_len), n)
+    if sm_scale is None:
+        sm_scale = d ** -0.5
+    lib = _lib.load()
+    with _on(dev):
+        if ws is None:
+            ws = workspace(lib.kessie_cross_attention_workspace_bytes(b, mq, t, hq, hkv, d, mk, dt), dev, "cross")
+        _lib.check("kessie_cross_attention", lib.kessie_cross_attention(
+            _ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1),
+            _ptr(_contig(query_start_loc, "query_start_loc")), _ptr(_contig(kv_start, "kv_start")),
+            _ptr(_contig(kv_lens, "kv_lens")), _ptr(key_mask), _ptr(out), out.stride(0), out.stride(1), b, mq, mk, t, n,
+            hq, hkv, d, float(sm_scale), dt, _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size(),
+            _stream_ptr(stream, dev)))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Tables of an engine step
+# ---------------------------------------------------------------------------
+class StepTables(NamedTuple):
+    query_start_loc: torch.Tensor  # int32 [B+1]
+    seq_lens: torch.Tensor         # int32 [B]
+    slot_mapping: torch.Tensor     # int64 [rows]
+    positions: torch.Tensor        # int32 [rows]
+    taken: torch.Tensor            # int32 [1]
+
+
+def step_tables(block_table: torch.Tensor, computed_lens: torch.Tensor, new_lens: torch.Tensor, page_size: int,
+                num_token_rows: int, free_pages: Optional[torch.Tensor] = None,
+                free_count: Optional[torch.Tensor] = None, position_delta: Optional[torch.Tensor] = None,
+                page_valid: Optional[torch.Tensor] = None, page_positions: Optional[torch.Tensor] = None,
+                out=None, stream=None) -> StepTables:
+    """The tables of one engine step from the requests' lengths, in one launch.
+
+    Request b holds computed_lens[b] tokens in the pages of block_table[b]
+    (int32 [B, W], updated in place) and brings new_lens[b] more (int32 [B]
+    each, negative counts as 0); the pages it needs are taken from the front of
+    free_pages (int32, the first free_count[0] of it -- what page_evict_list and
+    page_select_evict return) in request order.  A request whose pages or token
+    rows do not fit gets none: its slots are -1 and its seq_len stays
+    computed_lens[b].  The num_token_rows rows past the last token have slot -1
+    and position 0; positions count from computed_lens[b] + position_delta[b].
+    page_valid (int8) and page_positions (int32), if given, are set to 1 and to
+    the page's first position for the pages taken.
+
+    ``out``: a StepTables (or tuple of its five tensors) to fill again."""
+    if block_table.dtype != torch.int32 or computed_lens.dtype != torch.int32 or new_lens.dtype != torch.int32:
+        raise TypeError("block_table, computed_lens and new_lens must be int32")
+    b = computed_lens.numel()
+    if block_table.dim() != 2 or block_table.shape[0] < b or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be [B, W] with contiguous rows")
+    if new_lens.numel() != b:
+        raise ValueError("computed_lens and new_lens differ in length")
+    if page_size <= 0 or num_token_rows < 0:
+        raise ValueError(f"page_size {page_size}, num_token_rows {num_token_rows}")
+    max_free = num_pages = 0
+    if free_pages is not None:
+        if free_count is None:
+            raise ValueError("free_pages without free_count")
+        if free_pages.dtype != torch.int32 or free_count.dtype != torch.int32 or free_count.numel() < 1:
+            raise TypeError("free_pages and free_count must be int32")
+        max_free = free_pages.numel()
+    if position_delta is not None and (position_delta.dtype != torch.int32 or position_delta.numel() != b):
+        raise ValueError("position_delta must be int32 with one entry per request")
+    if page_valid is not None:
+        if page_valid.dtype != torch.int8:
+            raise TypeError("page_valid must be int8")
+        num_pages = page_valid.numel()
+    if page_positions is not None:
+        if page_positions.dtype != torch.int32:
+            raise TypeError("page_positions must be int32")
+        if page_valid is not None and page_positions.numel() != num_pages:
+            raise ValueError("page_valid and page_positions differ in length")
+        num_pages = page_positions.numel()
+    dev = block_table.device
+    if out is None:
+        ints = torch.empty(2 * b + 2 + num_token_rows, dtype=torch.int32, device=dev)
+        out = StepTables(ints[:b + 1], ints[b + 1:2 * b + 1], torch.empty(num_token_rows, dtype=torch.int64, device=dev),
+                         ints[2 * b + 2:], ints[2 * b + 1:2 * b + 2])
+    else:
+        out = out if type(out) is StepTables else StepTables(*out)
+        for name, t, dt, n in zip(StepTables._fields, out, (torch.int32, torch.int32, torch.int64, torch.int32, torch.int32),
+                                  (b + 1, b, num_token_rows, num_token_rows, 1)):
+            if t.dtype != dt or t.numel() != n or not t.is_contiguous():
+                raise ValueError(f"out.{name} must be a contiguous {dt} tensor of {n} entries")
+    _one_device(dev, computed_lens=computed_lens, new_lens=new_lens, free_pages=free_pages, free_count=free_count,
+                position_delta=position_delta, page_valid=page_valid, page_positions=page_positions, **out._asdict())
+    for name, t in (("computed_lens", computed_lens), ("new_lens", new_lens), ("free_pages", free_pages),
+                    ("position_delta", position_delta), ("page_valid", page_valid), ("page_positions", page_positions)):
+        if t is not None:
+            _contig(t, name)
+    with _on(dev):
+        _lib.check("kessie_step_tables", _lib.load().kessie_step_tables(
+            _ptr(block_table), block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1],
+            block_table.shape[1], _ptr(computed_lens), _ptr(new_lens),
+            _ptr(position_delta), _ptr(free_pages) if max_free else None, _ptr(free_count), max_free, b, int(page_size),
+            int(num_token_rows), _ptr(out[0]), _ptr(out[1]), _ptr(out[2]), _ptr(out[3]), _ptr(out[4]), _ptr(page_valid),
+            _ptr(page_positions), num_pages, _stream_ptr(stream, dev)))
+    return out
 
 
 # ---------------------------------------------------------------------------
