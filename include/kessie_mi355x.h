@@ -380,9 +380,11 @@ int kessie_rope_remap_axes(void* kv_pool, int64_t page_stride,
 /* Bytes of workspace kessie_cross_attention may need for these sizes (host
  * call). */
 size_t kessie_cross_attention_workspace_bytes(int batch, int max_query_len,
-                                              int num_q_tokens, int num_q_heads,
-                                              int num_kv_heads, int head_dim,
-                                              int max_kv_len, int dtype);
+                                              int num_q_tokens,
+                                              int num_kv_tokens,
+                                              int num_q_heads, int num_kv_heads,
+                                              int head_dim, int max_kv_len,
+                                              int dtype);
 
 /* Attention of each sequence's queries over its own encoder states, all of
  * them (no causal order, no window), GQA as in decode:

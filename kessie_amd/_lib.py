@@ -87,8 +87,8 @@ SIGNATURES = {
     # adjacent, T, H, D, R, P, dtype, stream
     "kessie_rope_remap_axes": (_I, [
         _P, _I64, _I64, _I64, _P, _I, _P, _I64, _P, _I64, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
-    # cross attention: B, max_q, T, Hq, Hkv, D, max_kv, dtype
-    "kessie_cross_attention_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    # cross attention: B, max_q, Tq, Tkv, Hq, Hkv, D, max_kv, dtype
+    "kessie_cross_attention_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I, _I]),
     # q + 2 strides, k + 2, v + 2, q_start, kv_start, kv_lens, mask, out + 2, B, max_q, max_kv, Tq, Tkv, Hq, Hkv, D,
     # sm_scale, dtype, ws, ws_bytes, stream
     "kessie_cross_attention": (_I, [

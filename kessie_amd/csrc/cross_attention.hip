@@ -63,9 +63,11 @@ struct Args {
   // at a scale of zero); a negative scale flips q instead (flip).
   float c2;
   int flip;
-  // Split partials, per row t * Hq + h and split: unnormalised sums [rows][S][D], base-2
-  // maxima and sums [rows][S].
-  int S;
+  // Work split over the states: `shares` workgroups per kv head wanted, each of at least
+  // min_steps steps.  plan: what the main kernel's first workgroup leaves for the merge.  Partials
+  // of part_rows rows each: unnormalised sums [rows][D], base-2 maxima and sums.
+  int shares, min_steps, part_rows;
+  int64_t* plan;
   float* ws_o;
   float* ws_m;
   float* ws_l;
@@ -96,6 +98,10 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // has no output registers; wait_loads is what it is waited for with.
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, uint32_t voff, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
+}
+// The same for what is read once (non-temporal).
+__device__ __forceinline__ void stream_to_lds(i32x4 rsrc, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
 }
 // All but the last n loads done.
 template <int n>
@@ -261,11 +267,15 @@ struct Core {
     }
     return sum;
   }
-  // Scores of hidden states (bits of `seen` not set: 32 states) become -inf.
+  // Scores of hidden states (bits of `seen` not set: 32 states) become -inf: the bit as a word of ones (a signed
+  // bit-field read), then a select by it.
   static __device__ __forceinline__ void hide(f32x16& s, uint32_t seen, int half) {
-    const uint32_t mine = seen >> (4 * half);
+    const int mine = (int)(seen >> (4 * half));
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = (mine >> (8 * (i / 4) + i % 4)) & 1 ? s[i] : kNegInf;
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t keep = (uint32_t)((mine << (31 - (8 * (i / 4) + i % 4))) >> 31);
+      s[i] = __uint_as_float((__float_as_uint(s[i]) & keep) | (0xff800000u & ~keep));
+    }
   }
   static __device__ __forceinline__ float top(const f32x16& s) {
     float m = s[0];
@@ -282,7 +292,13 @@ struct Core {
     for (int i = 0; i < QN; ++i) {
       q[i] = QV{};
       if (ok) q[i] = *reinterpret_cast<const QV*>(at + q_elem(i, half));
-      if (a.flip) q[i] = -q[i];
+    }
+  }
+  // A negative sm_scale (after the first tiles are asked for: it waits for q).
+  static __device__ __forceinline__ void flip_q(const Args& a, QV (&q)[QN]) {
+    if (a.flip) {
+#pragma unroll
+      for (int i = 0; i < QN; ++i) q[i] = -q[i];
     }
   }
 };
@@ -331,6 +347,213 @@ struct Seen {
   }
 };
 
+// One stretch of a workgroup's work: steps t .. end - 1 of row tile rt of sequence b.
+struct Stretch {
+  int b, rt, t, end, steps;  // steps: of the whole row tile
+  Seq sq;
+};
+
+// The row tiles and steps of sequence s (a sequence without states has one step, which stores its zeros).
+__device__ __forceinline__ int row_tiles(const Args& a, const Seq& s, int rows) { return div_up(s.nq * a.G, rows); }
+__device__ __forceinline__ int steps_of(const Seq& s, int keys) { return max(div_up(s.nkv, keys), 1); }
+
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return (int64_t)(((uint64_t)(uint32_t)uniform((int)((uint64_t)x >> 32)) << 32) | (uint32_t)uniform((int)(uint32_t)x));
+}
+__device__ __forceinline__ Seq uniform_sequence(const Args& a, int b) {
+  Seq s = sequence(a, b);
+  s.q0 = uniform(s.q0), s.nq = uniform(s.nq), s.kv0 = uniform(s.kv0), s.nkv = uniform(s.nkv);
+  return s;
+}
+
+// Shared work.  All (sequence, row tile, step) of a kv head in a row, `all` of
+// them, are dealt out evenly: workgroup j of n takes all * j / n .. all * (j +
+// 1) / n - 1, so lengths of any mix end together.  A row tile that lies in one
+// workgroup is stored by it; of the others each workgroup holds a partial --
+// number 1 of the tile it begins, 0 of the one that it goes on with -- and
+// cross_combine_kernel merges them in order.
+struct Share {
+  int64_t all;
+  int n;
+};
+__device__ __forceinline__ Share share_of(const Args& a, int64_t all) {
+  const int64_t n = all / a.min_steps;
+  return {all, (int)(n < 1 ? 1 : n < a.shares ? n : a.shares)};
+}
+// The workgroup that takes step x.
+__device__ __forceinline__ int owner(const Share& s, int64_t x) {
+  const uint64_t v = (uint64_t)((x + 1) * s.n - 1);
+  return (v | (uint64_t)s.all) >> 32 ? (int)(v / (uint64_t)s.all) : (int)((uint32_t)v / (uint32_t)s.all);
+}
+
+// The partial row of this workgroup's row r: of the tile it begins, or goes on with.
+__device__ __forceinline__ int64_t part_row(const Args& a, bool begins, int r) {
+  return ((int64_t)blockIdx.x * 2 + begins) * a.part_rows + r;
+}
+
+// Walks the stretches of a workgroup.
+template <bool kShare>
+struct Walk {
+  int64_t left;
+  Stretch now;
+
+  // False: nothing to do.  x: the workgroup's number among its kv head's.
+  __device__ __forceinline__ bool begin(const Args& a, int x, int rows, int keys, int lane) {
+    // Without sharing, workgroup x takes the x-th row tile of all; with it, the stretch from its first step.
+    int64_t before = 0, at = x, count = 1, all = 0;
+    if (kShare) {
+      for (int b0 = 0; b0 < a.B; b0 += 64) {
+        int64_t w = 0;
+        if (b0 + lane < a.B) {
+          const Seq s = sequence(a, b0 + lane);
+          w = (int64_t)row_tiles(a, s, rows) * steps_of(s, keys);
+        }
+        int64_t inc = w;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int64_t y = __shfl_up(inc, o, 64);
+          if (lane >= o) inc += y;
+        }
+        if (blockIdx.x == 0 && b0 + lane < a.B && threadIdx.x < 64) a.plan[b0 + lane] = all + inc - w;
+        all += __shfl(inc, 63, 64);
+      }
+      if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[a.B] = all;
+      const Share s = share_of(a, all);
+      if (x >= s.n) return false;
+      at = all * x / s.n;
+      count = all * (x + 1) / s.n - at;
+    }
+    at = uniform64(at);
+    left = uniform64(count);
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      int64_t w = 0;
+      if (b0 + lane < a.B) {
+        const Seq s = sequence(a, b0 + lane);
+        w = (int64_t)row_tiles(a, s, rows) * (kShare ? steps_of(s, keys) : 1);
+      }
+      int64_t inc = w;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int64_t y = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += y;
+      }
+      const int64_t total = __shfl(inc, 63, 64);
+      if (at < before + total) {
+        const int l = __ffsll((unsigned long long)__ballot(before + inc > at)) - 1;
+        const int off = uniform((int)(at - before - __shfl(inc - w, l, 64)));
+        now.b = uniform(b0 + l);
+        now.sq = uniform_sequence(a, now.b);
+        now.steps = steps_of(now.sq, keys);
+        now.rt = kShare ? uniform(off / now.steps) : off;
+        now.t = kShare ? uniform(off - now.rt * now.steps) : 0;
+        cut();
+        return true;
+      }
+      before += total;
+    }
+    return false;
+  }
+  __device__ __forceinline__ void cut() {
+    now.end = kShare ? (int)min((int64_t)now.steps, now.t + left) : now.steps;
+    if (kShare) left -= now.end - now.t;
+  }
+  // On to the next stretch; false: done.
+  __device__ __forceinline__ bool next(const Args& a, int rows, int keys) {
+    if (!kShare || left <= 0) return false;
+    now.t = 0;
+    if (++now.rt >= row_tiles(a, now.sq, rows)) {
+      now.rt = 0;
+      do {
+        now.sq = uniform_sequence(a, ++now.b);
+      } while (now.sq.nq == 0);  // (there is one: work is left)
+      now.steps = steps_of(now.sq, keys);
+    }
+    cut();
+    return true;
+  }
+};
+
+// The same value for the compiler's eyes too (loop-carried values would stay in vector registers).
+__device__ __forceinline__ Stretch uniform(const Stretch& s) {
+  return {uniform(s.b), uniform(s.rt), uniform(s.t), uniform(s.end), uniform(s.steps),
+          {uniform(s.sq.q0), uniform(s.sq.nq), uniform(s.sq.kv0), uniform(s.sq.nkv)}};
+}
+
+// Pieces of the tile kernel: each row tile of a sequence is cut into
+// ceil(steps / limit) stretches of equal length, one workgroup a stretch.
+struct Piece {
+  int rt, t, end, steps, pieces;
+  int first;  // number of the row tile's first piece
+  Seq sq;
+};
+// Lane l's sequence of the 64 from b0 on (none: no rows).
+__device__ __forceinline__ Seq lane_sequence(const Args& a, int b0, int lane) {
+  return b0 + lane < a.B ? sequence(a, b0 + lane) : Seq{0, 0, 0, 0};
+}
+// Finds the x-th piece of a kv head, or with kMerge its x-th row tile; false: there is none.  limit < 0: to be found
+// first, the longest stretch: an even share of the work.  One load of the lengths for up to 64 sequences.
+template <bool kMerge>
+__device__ __forceinline__ bool find_piece(const Args& a, int x, int rows, int keys, int& limit, int lane, Piece& p) {
+  Seq mine = lane_sequence(a, 0, lane);
+  if (limit < 0) {
+    float work = 0.0f, tiles = 0.0f;  // (fp32: every workgroup comes to the same limit, exact or not)
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      if (b0 > 0) mine = lane_sequence(a, b0, lane);
+      float n = (float)row_tiles(a, mine, rows), w = n * (float)steps_of(mine, keys);
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) {
+        w += __shfl_xor(w, o, 64);
+        n += __shfl_xor(n, o, 64);
+      }
+      work += w;
+      tiles += n;
+    }
+    if (a.B > 64) mine = lane_sequence(a, 0, lane);
+    // (ceil, and a little more for what the sums were rounded off: at most `shares` pieces and one a row tile.)
+    limit = uniform(max((int)fminf(ceilf(work / (float)a.shares * 1.0001f), 1.0e9f), a.min_steps));
+  }
+  // Long pieces (more than half the limit) are numbered first, so that the short ones fill the end.
+  int before = 0;
+#pragma unroll 1
+  for (int cls = 0; cls < (limit ? 2 : 1); ++cls) {
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      if (a.B > 64) mine = lane_sequence(a, b0, lane);
+      const int steps = steps_of(mine, keys), c = limit ? div_up(steps, limit) : 1;
+      const bool here = !limit || (2 * div_up(steps, c) > limit) == (cls == 0);
+      const int n = here ? row_tiles(a, mine, rows) : 0;
+      int inc = n * c;
+      [[maybe_unused]] int tiles = n;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += y;
+        if (kMerge) {
+          const int z = __shfl_up(tiles, o, 64);
+          if (lane >= o) tiles += z;
+        }
+      }
+      const int total = __builtin_amdgcn_readlane(kMerge ? tiles : inc, 63);
+      if (x < total) {
+        const int l = __ffsll((unsigned long long)__ballot((kMerge ? tiles : inc) > x)) - 1;
+        const int off = x - __builtin_amdgcn_readlane(kMerge ? tiles - n : inc - n * c, l);
+        p.sq = Seq{__builtin_amdgcn_readlane(mine.q0, l), __builtin_amdgcn_readlane(mine.nq, l), __builtin_amdgcn_readlane(mine.kv0, l),
+                   __builtin_amdgcn_readlane(mine.nkv, l)};
+        p.steps = steps_of(p.sq, keys);
+        p.pieces = __builtin_amdgcn_readlane(c, l);
+        p.rt = kMerge ? off : uniform(off / p.pieces);
+        p.first = before + __builtin_amdgcn_readlane(inc - n * c, l) + p.rt * p.pieces;
+        const int i = kMerge ? 0 : off - p.rt * p.pieces, per = uniform(div_up(p.steps, p.pieces));
+        p.t = i * per;
+        p.end = min(p.t + per, p.steps);
+        return true;
+      }
+      x -= total;
+      before += __builtin_amdgcn_readlane(inc, 63);
+    }
+  }
+  return false;
+}
+
 // Stores O^T of a row from the accumulators: element 32 db + 8 (i / 4) + 4 half + i % 4 in register i.
 template <typename T, int D>
 __device__ __forceinline__ void store_row(T* row, const f32x16 (&o)[D / 32], float by, int half) {
@@ -346,11 +569,10 @@ __device__ __forceinline__ void store_row(T* row, const f32x16 (&o)[D / 32], flo
     }
 }
 
-// Up to 32 rows of a (sequence, kv head): decoding.  Every wave streams tiles
-// of its own (wave w of split s takes tiles s * NW + w, + S * NW, ...) through
-// two LDS stages of its own, the next tile in flight while one is computed: no
-// barrier before the merge.  Bound: HBM.
-template <typename T, int D, int KT, int NW, bool kMask, bool kSplit>
+// Up to 32 rows of a (sequence, kv head): decoding.  A step is NW tiles, one a
+// wave; every wave streams its tiles through two LDS stages of its own, the next
+// tile in flight while one is computed: no barrier before the merge.  Bound: HBM.
+template <typename T, int D, int KT, int NW, bool kMask, bool kShare>
 __global__ __launch_bounds__(NW * 64) void cross_rows_kernel(Args a) {
   typedef Core<T, D> C;
   constexpr int NB = KT / 32;            // 32-state blocks of a tile
@@ -360,23 +582,25 @@ __global__ __launch_bounds__(NW * 64) void cross_rows_kernel(Args a) {
   extern __shared__ __align__(16) unsigned char smem[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(KESSIE_LDS unsigned char*)smem;
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
-  const int g = blockIdx.x % a.Hkv, unit = blockIdx.x / a.Hkv;
-  const int b = kSplit ? unit / a.S : unit, split = kSplit ? unit - b * a.S : 0;
-  const Seq sq = sequence(a, b);
-  const int rows = sq.nq * a.G;
-  if (rows == 0) return;
-  typename C::QV q[C::QN];
-  C::load_q(a, sq, min(col, rows - 1), g, half, q, col < rows);
-
+  const int g = blockIdx.x % a.Hkv;
   const int ts_k = (int)a.k_ts * (int)sizeof(T), ts_v = (int)a.v_ts * (int)sizeof(T);
-  const char* kbase = static_cast<const char*>(a.k) + ((int64_t)sq.kv0 * a.k_ts + (int64_t)g * a.k_hs) * (int64_t)sizeof(T);
-  const char* vbase = static_cast<const char*>(a.v) + ((int64_t)sq.kv0 * a.v_ts + (int64_t)g * a.v_hs) * (int64_t)sizeof(T);
-  const int tiles = div_up(sq.nkv, KT), first = split * NW + wave, step = a.S * NW;
-  const int n = tiles > first ? (tiles - first + step - 1) / step : 0;
-  Seen<kMask, KT> seen{kMask ? a.mask + sq.kv0 : nullptr, sq.nkv, first, step, 0};
-  const uint32_t mine = lds0 + (uint32_t)wave * 4 * kTile;  // this wave's stages: K, V, K, V
+  Walk<kShare> walk;
+  if (!walk.begin(a, blockIdx.x / a.Hkv, 32, NW * KT, lane)) return;
   C core;
   core.init(lane);
+  do {
+  const Stretch now = uniform(walk.now);
+  const Seq sq = now.sq;
+  const int rows = sq.nq * a.G;
+  typename C::QV q[C::QN];
+  C::load_q(a, sq, min(col, rows - 1), g, half, q, col < rows);
+  const char* kbase = static_cast<const char*>(a.k) + ((int64_t)sq.kv0 * a.k_ts + (int64_t)g * a.k_hs) * (int64_t)sizeof(T);
+  const char* vbase = static_cast<const char*>(a.v) + ((int64_t)sq.kv0 * a.v_ts + (int64_t)g * a.v_hs) * (int64_t)sizeof(T);
+  const int nkv = (int)min((int64_t)sq.nkv, (int64_t)now.end * (NW * KT));  // states up to this stretch's end
+  const int first = now.t * NW + wave, step = NW;
+  const int n = uniform(max(div_up(div_up(nkv, KT) - first, step), 0));
+  Seen<kMask, KT> seen{kMask ? a.mask + sq.kv0 : nullptr, nkv, first, step, 0};
+  const uint32_t mine = lds0 + (uint32_t)wave * 4 * kTile;  // this wave's stages: K, V, K, V
 
   uint64_t bits[2];
   auto issue = [&](int t, int stage) {
@@ -387,13 +611,13 @@ __global__ __launch_bounds__(NW * 64) void cross_rows_kernel(Args a) {
     const i32x4 vr = tile_rsrc(vbase + (int64_t)tile * KT * ts_v, r, ts_v, C::RB);
     const uint32_t to = mine + (uint32_t)stage * 2 * kTile;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) load_to_lds(kr, C::k_offset(i, lane, ts_k), uniform(to + 1024u * i));
+    for (int i = 0; i < NI; ++i) stream_to_lds(kr, C::k_offset(i, lane, ts_k), uniform(to + 1024u * i));
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       uint32_t off = C::v_offset(i, lane, ts_v);
       // (A hidden state's V arrives as zeros, whatever it holds.)
       if (kMask && !((at >> (i * C::RPI + lane / C::CH)) & 1)) off = 0xffffff00u;
-      load_to_lds(vr, off, uniform(to + kTile + 1024u * i));
+      stream_to_lds(vr, off, uniform(to + kTile + 1024u * i));
     }
   };
 
@@ -434,6 +658,7 @@ __global__ __launch_bounds__(NW * 64) void cross_rows_kernel(Args a) {
   if (n > 0) {
     issue(0, 0);
     issue(1, 1);
+    C::flip_q(a, q);
     for (int t = 0; t < n; t += 2) {
       tile(t, 0);
       if (t + 1 < n) tile(t + 1, 1);
@@ -469,8 +694,8 @@ __global__ __launch_bounds__(NW * 64) void cross_rows_kernel(Args a) {
       if (e != 0.0f) y += e * *reinterpret_cast<const f32x4*>(so + (w * 32 + r) * kOut + d);
     }
     const int pos = (unsigned)r / (unsigned)a.G, h = g * a.G + r - pos * a.G;
-    if constexpr (kSplit) {
-      const int64_t row = ((int64_t)(sq.q0 + pos) * a.Hq + h) * a.S + split;
+    if (kShare && !(now.t == 0 && now.end == now.steps)) {
+      const int64_t row = part_row(a, now.t == 0, r);
       *reinterpret_cast<f32x4*>(a.ws_o + row * D + d) = y;
       if (d == 0) {
         a.ws_m[row] = top;
@@ -485,20 +710,19 @@ __global__ __launch_bounds__(NW * 64) void cross_rows_kernel(Args a) {
       *reinterpret_cast<V*>(static_cast<T*>(a.out) + (int64_t)(sq.q0 + pos) * a.o_ts + (int64_t)h * a.o_hs + d) = z;
     }
   }
+  if (kShare) __syncthreads();  // (the next stretch loads over the merge)
+  } while (walk.next(a, 32, NW * KT));
 }
 
 // max(a, b, c) in one instruction (fmaxf on MFMA results first quiets each
 // input).  Inline assembly gets no wait states from the compiler's MFMA hazard
-// checks: its uses read scores whose MFMAs lie a whole PV product back, or
-// settle() them first.
+// checks (a 32x32 result needs 18): its use reads scores four MFMAs after the
+// last one that wrote them.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
-// 24 wait states after the MFMAs that wrote s (a 32x32 result needs 18).
-__device__ __forceinline__ void settle(f32x16& s) { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(s)); }
-
 // Headroom of the lazy rescale, in log2 units: probabilities up to 2^8, as
 // exact in either type as any up to 1; the O accumulators move only when a row's
 // maximum rises by more.
@@ -510,7 +734,7 @@ constexpr float kSlack = 8.0f;
 // softmax of tile t in the shadow of S^T(t + 1), then O^T += V^T P^T(t); one
 // barrier.  Each MFMA is issued with its share of the other work and its
 // operands two steps ahead, in a fixed order (a scheduling barrier a step).
-template <typename T, int D, int W, bool kMask, bool kSplit>
+template <typename T, int D, int W, bool kMask, bool kShare>
 __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void cross_tile_kernel(Args a) {
   typedef Core<T, D> C;
   typedef typename C::QV QV;
@@ -522,40 +746,12 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   const uint32_t lds0 = (uint32_t)(uintptr_t)(KESSIE_LDS unsigned char*)smem;
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
   const int g = blockIdx.x % a.Hkv;
-  int rt = blockIdx.x / a.Hkv;
-  // x / Hkv numbers the live (sequence, row tile) pairs in order; the grid's surplus ends here.
-  int b = -1;
-  for (int b0 = 0, before = 0; b0 < a.B; b0 += 64) {
-    const int nt = b0 + lane < a.B ? div_up(sequence(a, b0 + lane).nq * a.G, kRows) : 0;
-    int inc = nt;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(inc, o, 64);
-      if (lane >= o) inc += y;
-    }
-    const int total = __builtin_amdgcn_readlane(inc, 63);
-    if (rt < before + total) {
-      const int l = __ffsll((unsigned long long)__ballot(before + inc > rt)) - 1;
-      b = uniform(b0 + l);
-      rt = uniform(rt - before - __builtin_amdgcn_readlane(inc - nt, l));
-      break;
-    }
-    before += total;
-  }
-  if (b < 0) return;
-  Seq sq = sequence(a, b);
-  sq.q0 = uniform(sq.q0), sq.nq = uniform(sq.nq), sq.kv0 = uniform(sq.kv0), sq.nkv = uniform(sq.nkv);
-  const int rows = sq.nq * a.G, row = rt * kRows + wave * 32 + col;
-  QV q[C::QN];
-  C::load_q(a, sq, min(row, rows - 1), g, half, q, row < rows);
-
   const int ts_k = (int)a.k_ts * (int)sizeof(T), ts_v = (int)a.v_ts * (int)sizeof(T);
-  const char* kbase = static_cast<const char*>(a.k) + ((int64_t)sq.kv0 * a.k_ts + (int64_t)g * a.k_hs) * (int64_t)sizeof(T);
-  const char* vbase = static_cast<const char*>(a.v) + ((int64_t)sq.kv0 * a.v_ts + (int64_t)g * a.v_hs) * (int64_t)sizeof(T);
-  const int split = kSplit ? (int)blockIdx.z : 0, S = kSplit ? a.S : 1;
-  const int tiles = div_up(sq.nkv, KT);
-  const int n = uniform(tiles > split ? (tiles - split + S - 1) / S : 0);
-  Seen<kMask, KT> seen{kMask ? a.mask + sq.kv0 : nullptr, sq.nkv, split, S, 0};
+  int limit = kShare ? -1 : 0;
+  Piece now;
+  const bool some = find_piece<false>(a, blockIdx.x / a.Hkv, kRows, KT, limit, lane, now);
+  if (kShare && blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int32_t*>(a.plan) = limit;
+  if (!some) return;
   C core;
   core.init(lane);
   uint32_t ko[NI], vo[NI];
@@ -564,14 +760,37 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     ko[i] = C::k_offset(wave + W * i, lane, ts_k);
     vo[i] = C::v_offset(wave + W * i, lane, ts_v);
   }
-  // Stages: K, K, V, V.
+  const Seq sq = now.sq;
+  const int rows = sq.nq * a.G, row = now.rt * kRows + wave * 32 + col;
+  QV q[C::QN];
+  C::load_q(a, sq, min(row, rows - 1), g, half, q, row < rows);
+  const char* kbase = static_cast<const char*>(a.k) + ((int64_t)sq.kv0 * a.k_ts + (int64_t)g * a.k_hs) * (int64_t)sizeof(T);
+  const char* vbase = static_cast<const char*>(a.v) + ((int64_t)sq.kv0 * a.v_ts + (int64_t)g * a.v_hs) * (int64_t)sizeof(T);
+  const int first = now.t, nkv = (int)min((int64_t)sq.nkv, (int64_t)now.end * KT);
+  const int n = uniform(max(div_up(nkv, KT) - first, 0));
+  auto rows_of = [&](int t) { return min(max(nkv - (first + t) * KT, 0), KT); };
+  // The states of a tile that are there and not hidden, one bit each; the mask's bytes are loaded a tile ahead.
+  auto mask_byte = [&](int t) {
+    const int j = (first + t) * KT + lane;
+    return kMask && j < nkv ? (int)a.mask[(int64_t)sq.kv0 + j] : 0;
+  };
+  auto seen = [&](int t, int byte) {
+    const int n = rows_of(t);
+    const uint64_t there = n >= 64 ? ~0ull : (1ull << n) - 1ull;
+    return kMask ? there & __builtin_amdgcn_ballot_w64(byte != 0) : there;
+  };
+  // Stages: K, K, V, V.  Tiles are loaded in order: the next one's place is carried along.
+  const char* kp = kbase + (int64_t)first * KT * ts_k;
+  const char* vp = vbase + (int64_t)first * KT * ts_v;
   auto issue_k = [&](int t, int stage) {
-    const i32x4 r = tile_rsrc(kbase + (int64_t)(split + t * S) * KT * ts_k, seen.rows(t), ts_k, C::RB);
+    const i32x4 r = tile_rsrc(kp, rows_of(t), ts_k, C::RB);
+    kp += KT * ts_k;
 #pragma unroll
     for (int i = 0; i < NI; ++i) load_to_lds(r, ko[i], uniform(lds0 + stage * kTile + 1024u * (wave + W * i)));
   };
   auto issue_v = [&](int t, int stage, uint64_t bits) {
-    const i32x4 r = tile_rsrc(vbase + (int64_t)(split + t * S) * KT * ts_v, seen.rows(t), ts_v, C::RB);
+    const i32x4 r = tile_rsrc(vp, rows_of(t), ts_v, C::RB);
+    vp += KT * ts_v;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       uint32_t off = vo[i];
@@ -585,26 +804,23 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   for (int i = 0; i < C::DB; ++i) o[i] = f32x16{};
   float m = kNegInf, l = 0.0f;
   const float c2 = a.c2;
-  uint64_t now = 0, next = 0;  // states of tiles t and t + 1
-  auto iteration = [&](int t, f32x16 (&s)[2], f32x16 (&sn)[2], const int par) {
+  uint64_t bits = 0, bits1 = 0;  // the states of tiles t and t + 1
+  int byte = 0;                  // this lane's mask byte of tile t + 2
+  float high = 0.0f;             // this lane's largest score of tile t, before any are hidden
+  auto iteration = [&](int t, f32x16 (&s)[2], f32x16 (&sn)[2], const int par) {  // par = t % 2
+    const uint64_t bits2 = seen(t + 2, byte);
+    byte = mask_byte(t + 3);
     issue_k(t + 2, par);
-    issue_v(t + 1, par ^ 1, next);
+    issue_v(t + 1, par ^ 1, bits1);
     const uint32_t kn = lds0 + (par ^ 1) * kTile, vn = lds0 + (2 + par) * kTile;
-    if (now != ~0ull) {
-      C::hide(s[0], (uint32_t)now, half);
-      C::hide(s[1], (uint32_t)(now >> 32), half);
+    if (bits != ~0ull) {
+      C::hide(s[0], (uint32_t)bits, half);
+      C::hide(s[1], (uint32_t)(bits >> 32), half);
+      high = fmaxf(C::top(s[0]), C::top(s[1]));
     }
-    now = next;
-    next = seen.at(t + 2, lane);
-    float ma = s[0][0], mb = s[1][0];
-#pragma unroll
-    for (int i = 1; i < 15; i += 2) {
-      ma = max3(ma, s[0][i], s[0][i + 1]);
-      mb = max3(mb, s[1][i], s[1][i + 1]);
-    }
-    ma = max3(ma, s[0][15], mb);
-    ma = max3(ma, s[1][15], s[1][15]);
-    const float top = max_halves(ma) * c2;
+    bits = bits1;
+    bits1 = bits2;
+    const float top = max_halves(high) * c2;
     const float mn = top > m + kSlack ? top : m;
     const float use = mn == kNegInf ? 0.0f : mn;
     const float alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -623,17 +839,18 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         for (int i = 0; i < 16; ++i) s[nb][i] = __builtin_amdgcn_exp2f(fmaf(s[nb][i], c2, -use));
         l += core.add(vn + (uint32_t)(32 * nb * C::RB), s[nb], o);
       }
+      high = fmaxf(C::top(sn[0]), C::top(sn[1]));
     } else {
-      constexpr int kQ = 2 * C::QN, kPV = 4 * C::DB, kPairs = 16 / kQ;
+      // Steps: the MFMAs of S^T(t + 1), then those of PV, each with its operand two steps ahead and its share of the
+      // 16 score pairs, which go through three stages in three steps -- scaled; exp2; packed and summed -- so that no
+      // stage waits for the one before; a pair is packed before the PV step that takes it.  The last steps take the
+      // next tile's largest score.
+      constexpr int kQ = 2 * C::QN, kPV = 4 * C::DB, kSpread = kQ + 3 * C::DB - 2, kMaxAt = kQ + 4, kMaxPer = 16 / (kPV - 4) + (16 % (kPV - 4) != 0);
+      static_assert(kQ + 3 * C::DB >= kSpread + 2, "the last pairs are packed in time");
       u32x4 w[4];  // p as V^T's partner: w[c] of states 16 c ..
       float l0 = 0.0f, l1 = 0.0f;
-      auto exp_pair = [&](int j) {
-        const int nb = j >> 3, i = 2 * (j & 7);
-        const uint32_t x = pack2<T>(__builtin_amdgcn_exp2f(fmaf(s[nb][i], c2, -use)), __builtin_amdgcn_exp2f(fmaf(s[nb][i + 1], c2, -use)));
-        w[j >> 2][j & 3] = x;
-        if (j & 1) l1 = Half<T>::sum2(x, l1);
-        else l0 = Half<T>::sum2(x, l0);
-      };
+      float hi[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+      auto first_pair = [](int i) { return i < 0 ? 0 : i >= kSpread ? 16 : i * 16 / kSpread; };
       auto operand = [&](int i) {
         if (i < kQ) return core.k_read(kn + (uint32_t)(32 * (i & 1) * C::RB), i >> 1);
         const int j = i - kQ, c = j / C::DB;
@@ -652,28 +869,49 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
           o[j % C::DB] = Half<T>::mma(op[i % (kAhead + 1)], __builtin_bit_cast(QV, w[j / C::DB]), o[j % C::DB]);
         }
         if (i + kAhead < kQ + kPV) op[(i + kAhead) % (kAhead + 1)] = operand(i + kAhead);
-        if (i < kQ) {
 #pragma unroll
-          for (int e = 0; e < kPairs; ++e) exp_pair(i * kPairs + e);
+        for (int j = first_pair(i - 2); j < first_pair(i - 1); ++j) {
+          const int nb = j >> 3, e = 2 * (j & 7);
+          const uint32_t x = pack2<T>(s[nb][e], s[nb][e + 1]);
+          w[j >> 2][j & 3] = x;
+          if (j & 1) l1 = Half<T>::sum2(x, l1);
+          else l0 = Half<T>::sum2(x, l0);
         }
+#pragma unroll
+        for (int j = first_pair(i - 1); j < first_pair(i); ++j) {
+          const int nb = j >> 3, e = 2 * (j & 7);
+          s[nb][e] = __builtin_amdgcn_exp2f(s[nb][e]);
+          s[nb][e + 1] = __builtin_amdgcn_exp2f(s[nb][e + 1]);
+        }
+#pragma unroll
+        for (int j = first_pair(i); j < first_pair(i + 1); ++j) {
+          const int nb = j >> 3, e = 2 * (j & 7);
+          s[nb][e] = fmaf(s[nb][e], c2, -use);
+          s[nb][e + 1] = fmaf(s[nb][e + 1], c2, -use);
+        }
+#pragma unroll
+        for (int j = (i - kMaxAt) * kMaxPer; j < (i - kMaxAt + 1) * kMaxPer && j < 16; ++j)
+          if (j >= 0) hi[j & 3] = max3(hi[j & 3], sn[j & 1][j & ~1], sn[j & 1][j | 1]);
         __builtin_amdgcn_sched_barrier(0);
       }
       l += l0 + l1;
+      high = fmaxf(max3(hi[0], hi[1], hi[2]), hi[3]);
     }
     wait_loads_and_meet();
   };
   if (n > 0) {
-    now = seen.at(0, lane);
-    next = seen.at(1, lane);
+    bits = seen(0, mask_byte(0));
+    bits1 = seen(1, mask_byte(1));
+    byte = mask_byte(2);
     issue_k(0, 0);
-    issue_v(0, 0, now);
+    issue_v(0, 0, bits);
     issue_k(1, 1);
+    C::flip_q(a, q);
     wait_loads_and_meet();
     f32x16 sa[2], sb[2];
     sa[0] = core.scores(lds0, q);
     sa[1] = core.scores(lds0 + 32 * C::RB, q);
-    settle(sa[0]);
-    settle(sa[1]);
+    high = fmaxf(C::top(sa[0]), C::top(sa[1]));
     wait_loads_and_meet();  // (iteration 0 loads over tile 0's K)
     for (int t = 0; t < n; t += 2) {
       iteration(t, sa, sb, 0);
@@ -681,51 +919,133 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     }
   }
   l = sum_halves(l);
-  if (row >= rows) return;
-  const int pos = (unsigned)row / (unsigned)a.G, h = g * a.G + row - pos * a.G;
-  if constexpr (kSplit) {
-    const int64_t r = ((int64_t)(sq.q0 + pos) * a.Hq + h) * S + split;
-    store_row<float, D>(a.ws_o + r * D, o, 1.0f, half);
-    if (half == 0) {
-      a.ws_m[r] = m;
-      a.ws_l[r] = l;
+  if (row < rows) {
+    const int pos = (unsigned)row / (unsigned)a.G, h = g * a.G + row - pos * a.G;
+    if (!kShare || now.pieces == 1) {
+      store_row<T, D>(static_cast<T*>(a.out) + (int64_t)(sq.q0 + pos) * a.o_ts + (int64_t)h * a.o_hs, o, l != 0.0f ? 1.0f / l : 0.0f, half);
+    } else {
+      const int64_t r = (int64_t)blockIdx.x * a.part_rows + wave * 32 + col;
+      store_row<float, D>(a.ws_o + r * D, o, 1.0f, half);
+      if (half == 0) {
+        a.ws_m[r] = m;
+        a.ws_l[r] = l;
+      }
     }
-  } else {
-    store_row<T, D>(static_cast<T*>(a.out) + (int64_t)(sq.q0 + pos) * a.o_ts + (int64_t)h * a.o_hs, o, l != 0.0f ? 1.0f / l : 0.0f, half);
   }
 }
 
-// Merges the S partials of a row: one wave a (query, head), in split order.
+// Merges the pieces of 1024 / D rows of a row tile, in order, eight loads in flight.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void cross_combine_kernel(Args a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t item = n / a.Hq;
-  const int h = (int)(n - item * a.Hq), b = (int)(item / a.max_q), i = (int)(item - (int64_t)b * a.max_q);
-  if (b >= a.B) return;
-  const Seq s = sequence(a, b);
-  if (i >= s.nq) return;
-  const int64_t row = ((int64_t)(s.q0 + i) * a.Hq + h) * a.S;
-  float top = kNegInf;
-  for (int x = lane; x < a.S; x += 64) top = fmaxf(top, a.ws_m[row + x]);
+__global__ __launch_bounds__(256) void cross_merge_kernel(Args a, int rows_per, int keys) {
+  constexpr int kLanes = D / 4, kRows = 256 / kLanes, kAhead = 8;
+  const int lane = threadIdx.x & 63, d = 4 * (threadIdx.x % kLanes);
+  const int g = blockIdx.x % a.Hkv;
+  Piece p;
+  int limit = uniform(*reinterpret_cast<const int32_t*>(a.plan));
+  if (!find_piece<true>(a, blockIdx.x / a.Hkv, rows_per, keys, limit, lane, p) || p.pieces == 1) return;
+  const int rows = min(p.sq.nq * a.G - p.rt * rows_per, rows_per), r = blockIdx.y * kRows + threadIdx.x / kLanes;
+  if (r >= rows) return;
+  const int64_t at = ((int64_t)p.first * a.Hkv + g) * a.part_rows + r, step = (int64_t)a.Hkv * a.part_rows;
+  // The online form: a piece's maximum and sum with its values.
+  float top = kNegInf, sum = 0.0f;
+  f32x4 y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i0 = 0; i0 < p.pieces; i0 += kAhead) {
+    float m[kAhead], l[kAhead];
+    f32x4 v[kAhead];
 #pragma unroll
-  for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-  const float use = top == kNegInf ? 0.0f : top;
-  constexpr int N = D / 64;  // elements of a lane
-  float y[N] = {}, sum = 0.0f;
-  for (int x = 0; x < a.S; ++x) {
-    const float e = __builtin_amdgcn_exp2f(a.ws_m[row + x] - use);
-    sum += e * a.ws_l[row + x];
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t n = at + (int64_t)min(i0 + i, p.pieces - 1) * step;
+      m[i] = a.ws_m[n];
+      l[i] = a.ws_l[n];
+      v[i] = *reinterpret_cast<const f32x4*>(a.ws_o + n * D + d);
+    }
+    float mn = top;
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const float v = a.ws_o[(row + x) * D + lane * N + k];
-      if (e != 0.0f) y[k] += e * v;
+    for (int i = 0; i < kAhead; ++i) {
+      if (i0 + i >= p.pieces) m[i] = kNegInf;
+      mn = fmaxf(mn, m[i]);
+    }
+    const float use = mn == kNegInf ? 0.0f : mn, was = __builtin_amdgcn_exp2f(top - use);
+    sum *= was;
+    y *= was;
+    top = mn;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float e = __builtin_amdgcn_exp2f(m[i] - use);
+      if (e != 0.0f) {
+        sum += e * l[i];
+        y += e * v[i];
+      }
     }
   }
   const float il = sum != 0.0f ? 1.0f / sum : 0.0f;
-  T* out = static_cast<T*>(a.out) + (int64_t)(s.q0 + i) * a.o_ts + (int64_t)h * a.o_hs + lane * N;
+  const int row = p.rt * rows_per + r, pos = (unsigned)row / (unsigned)a.G, h = g * a.G + row - pos * a.G;
+  typedef T V __attribute__((ext_vector_type(4)));
+  V z;
 #pragma unroll
-  for (int k = 0; k < N; ++k) out[k] = from_f32<T>(y[k] * il);
+  for (int k = 0; k < 4; ++k) z[k] = from_f32<T>(y[k] * il);
+  *reinterpret_cast<V*>(static_cast<T*>(a.out) + (int64_t)(p.sq.q0 + pos) * a.o_ts + (int64_t)h * a.o_hs + d) = z;
+}
+
+// Merges the partials of rows that several workgroups share, in step order.  One
+// wave a query and `heads` of its heads; D / 4 lanes a row, so 64 / (D / 4) heads
+// at a time: the look-up of the sequence and its workgroups is shared by them.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cross_combine_kernel(Args a, int rows_per, int keys, int heads) {
+  constexpr int kLanes = D / 4, kAtOnce = 64 / kLanes;
+  const int lane = threadIdx.x & 63, sub = lane / kLanes, d = 4 * (lane % kLanes);
+  const int t = uniform((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+  if (t >= a.Tq) return;
+  // The sequence that row t belongs to: the last that starts at or before it.
+  const int q0 = a.q_start[0];
+  int b = -1;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const bool le = b0 + lane < a.B && a.q_start[b0 + lane] - q0 <= t;
+    const unsigned long long m = __ballot(le);
+    if (m == 0) break;
+    b = b0 + 63 - __clzll((long long)m);
+  }
+  b = uniform(b);
+  if (b < 0) return;
+  const Seq s = uniform_sequence(a, b);
+  const int i = t - s.q0;
+  if (i < 0 || i >= s.nq) return;
+  const Share sh = share_of(a, a.plan[a.B]);
+  const int steps = steps_of(s, keys);
+  const int64_t before = a.plan[b];
+  const int h_end = min(a.Hq, (int)(blockIdx.y + 1) * heads);
+  int last = -1, j0 = 0, j1 = 0;
+  for (int h0 = blockIdx.y * heads; h0 < h_end; h0 += kAtOnce) {
+    const int h = min(h0 + sub, h_end - 1), g = h / a.G, row = i * a.G + h - g * a.G, rt = row / rows_per;
+    const int64_t r = row - rt * rows_per;
+    if (__builtin_amdgcn_ballot_w64(rt != last) != 0) {  // (a query's heads lie in one row tile, or in two)
+      const int64_t x = before + (int64_t)rt * steps;
+      j0 = owner(sh, x), j1 = owner(sh, x + steps - 1);
+      last = rt;
+    }
+    if (j0 == j1 || h0 + sub >= h_end) continue;  // stored already
+    // Partial of workgroup j: number 1 of the first, 0 of those after it.
+    auto part = [&](int j) { return (((int64_t)j * a.Hkv + g) * 2 + (j == j0)) * a.part_rows + r; };
+    float top = kNegInf;
+    for (int j = j0; j <= j1; ++j) top = fmaxf(top, a.ws_m[part(j)]);
+    const float use = top == kNegInf ? 0.0f : top;
+    f32x4 y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int j = j0; j <= j1; ++j) {
+      const int64_t p = part(j);
+      const float e = __builtin_amdgcn_exp2f(a.ws_m[p] - use);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(a.ws_o + p * D + d);
+      sum += e * a.ws_l[p];
+      if (e != 0.0f) y += e * v;
+    }
+    const float il = sum != 0.0f ? 1.0f / sum : 0.0f;
+    typedef T V __attribute__((ext_vector_type(4)));
+    V z;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) z[k] = from_f32<T>(y[k] * il);
+    *reinterpret_cast<V*>(static_cast<T*>(a.out) + (int64_t)t * a.o_ts + (int64_t)h * a.o_hs + d) = z;
+  }
 }
 
 // Any head_dim up to 256, any strides and type: one wave per (query, head),
@@ -809,65 +1129,104 @@ int launch_lds(F kernel, const Args& a, dim3 grid, int threads, size_t lds, hipS
   return check_launch("cross attention");
 }
 
-// The grid: rows kernel or tile kernel, and the splits of the states.
+// The launch: which kernel, and whether the states are split.
 struct Plan {
-  bool few;       // cross_rows_kernel
-  int S;
-  int64_t tiles;  // workgroups per kv head and split
+  int waves;        // 0: cross_rows_kernel; 4, 8: cross_tile_kernel
+  int shares;       // workgroups wanted per kv head; 0: one a row tile, no partials
+  int64_t tiles;    // at least the row tiles of a kv head
+  int64_t grid;     // workgroups per kv head
+  int min_steps, part_rows;
 };
-constexpr int kRowsWaves = 4, kTileWaves = 4;
+constexpr int kRowsKeys = 32;
+// Waves of cross_rows_kernel: 32 KiB of LDS each, 64 at fp32 and head_dim 128.
 template <typename T, int D>
-constexpr int rows_kt() {
-  return 32;
+constexpr int rows_waves() {
+  return Core<T, D>::RB == 512 ? 2 : 4;
 }
-Plan make_plan(int B, int max_q, int Tq, int Hq, int Hkv, int D, int max_kv, int es) {
-  const int G = Hq / Hkv, cus = attn::device_cus();
-  Plan p;
-  p.few = (int64_t)max_q * G <= 32;
-  if (p.few) {
+Plan make_plan(int B, int max_q, int Tq, int Hq, int Hkv, int D, int max_kv, int Tkv, int es) {
+  const int G = Hq / Hkv, cus = attn::device_cus(), row_bytes = D * es;
+  const int64_t most = (int64_t)max_q * G;  // rows of a sequence
+  auto tiles_of = [&](int rows) {
+    const int64_t by_len = (int64_t)B * ((most + rows - 1) / rows), by_rows = (int64_t)Tq * G / rows + B;
+    return by_len < by_rows ? by_len : by_rows;
+  };
+  Plan p{};
+  int keys, per_cu, gain;
+  if (most <= 32) {
+    const int nw = row_bytes == 512 ? 2 : 4;
     p.tiles = B;
-    const int64_t units = (int64_t)B * Hkv;
-    const int waves_tiles = div_up(max_kv, 32 * kRowsWaves);  // tiles of a wave, unsplit
-    int64_t S = (2 * cus + units - 1) / units;
-    if (S > waves_tiles / 4) S = waves_tiles / 4;
-    p.S = S < 1 ? 1 : (int)S;
+    p.part_rows = (int)most;
+    p.min_steps = 2;
+    keys = nw * kRowsKeys;
+    per_cu = 160 * 1024 / (nw * 4 * kRowsKeys * row_bytes);
+    gain = 5;
   } else {
-    const int rows = kTileWaves * 32;
-    const int64_t by_len = (int64_t)B * (((int64_t)max_q * G + rows - 1) / rows), by_rows = (int64_t)Tq * G / rows + B;
-    p.tiles = by_len < by_rows ? by_len : by_rows;
-    const int64_t wgs = p.tiles * Hkv;
-    int64_t S = 2 * cus / wgs;
-    if (S > div_up(max_kv, 64) / 8) S = div_up(max_kv, 64) / 8;
-    p.S = S < 1 ? 1 : (int)S;
+    // Eight waves share a tile's load where that still gives every CU a workgroup: 4,096 queries on 16,384 (32 / 8
+    // heads of 128) 931 us against 1,015 with four; 8 x 200 on 1,000 (8 heads) 32.2 against 23.9.
+    p.waves = es == 2 && tiles_of(256) * Hkv >= cus ? 8 : 4;
+    const int rows = p.waves * 32;
+    p.tiles = tiles_of(rows);
+    p.part_rows = (int)(most < rows ? most : rows);
+    p.min_steps = es == 4 ? 2 : 4;
+    keys = 64;
+    per_cu = p.waves == 8 || row_bytes == 512 ? 1 : 2;
+    gain = es == 4 ? 4 : 14;
+  }
+  p.grid = p.tiles;
+  // Split where the longest sequence would outlast an even share of the work by more than the merge costs (`gain`
+  // steps: 5 us of it in decoding, 10 otherwise).  What an even share is goes by the means that the host knows.
+  const int64_t slots = (int64_t)cus * per_cu;
+  const double mean = B > 0 && Tkv / B < max_kv ? (double)Tkv / B : max_kv, tiles = (double)Tq * G / (p.waves ? p.waves * 32 : 32) + 0.5 * B;
+  const double even = (tiles < p.tiles ? tiles : (double)p.tiles) * Hkv * (mean / keys + 0.5) / (double)slots;
+  if (div_up(max_kv, keys) - even >= gain) {
+    p.shares = (int)((slots + Hkv - 1) / Hkv);
+    p.grid = p.waves ? p.shares + p.tiles : p.shares;
   }
   return p;
 }
 
-template <typename T, int D, bool kMask, bool kSplit>
+struct Layout {
+  size_t plan, rows, bytes;  // bytes of the plan, partial rows, all bytes
+};
+Layout layout(const Plan& p, int B, int Hkv, int D) {
+  Layout l{};
+  if (p.shares) {
+    l.plan = ((size_t)(B + 1) * 8 + 255) / 256 * 256;
+    l.rows = (size_t)p.grid * Hkv * (p.waves ? 1 : 2) * p.part_rows;
+    l.bytes = l.plan + l.rows * (D + 2) * sizeof(float);
+  }
+  return l;
+}
+
+template <typename T, int D, bool kMask, bool kShare>
 int launch_fast(const Args& a, const Plan& p, hipStream_t s) {
   typedef Core<T, D> C;
-  if (p.few) {
-    constexpr int KT = rows_kt<T, D>(), NW = C::RB == 512 ? 2 : kRowsWaves;
-    constexpr size_t stages = (size_t)NW * 4 * KT * C::RB, merge = (size_t)NW * 32 * (D + 4 + 2) * 4;
-    return launch_lds(cross_rows_kernel<T, D, KT, NW, kMask, kSplit>, a, dim3((unsigned)(p.tiles * a.Hkv * p.S)), NW * 64,
-                      stages > merge ? stages : merge, s);
+  const dim3 grid((unsigned)(p.grid * a.Hkv));
+  constexpr size_t tile = (size_t)4 * 64 * C::RB;
+  if constexpr (!C::kF32) {
+    if (p.waves == 8) return launch_lds(cross_tile_kernel<T, D, 8, kMask, kShare>, a, grid, 512, tile, s);
   }
-  constexpr int W = kTileWaves;
-  return launch_lds(cross_tile_kernel<T, D, W, kMask, kSplit>, a, dim3((unsigned)(p.tiles * a.Hkv), 1, p.S), W * 64, (size_t)4 * 64 * C::RB, s);
+  if (p.waves) return launch_lds(cross_tile_kernel<T, D, 4, kMask, kShare>, a, grid, 256, tile, s);
+  constexpr int KT = kRowsKeys, NW = rows_waves<T, D>();
+  constexpr size_t stages = (size_t)NW * 4 * KT * C::RB, merge = (size_t)NW * 32 * (D + 4 + 2) * 4;
+  return launch_lds(cross_rows_kernel<T, D, KT, NW, kMask, kShare>, a, grid, NW * 64, stages > merge ? stages : merge, s);
 }
 
 template <typename T, int D>
-int launch_split(const Args& a, const Plan& p, hipStream_t s) {
-  if (p.S == 1) return a.mask ? launch_fast<T, D, true, false>(a, p, s) : launch_fast<T, D, false, false>(a, p, s);
+int launch_shared(const Args& a, const Plan& p, hipStream_t s) {
+  if (!p.shares) return a.mask ? launch_fast<T, D, true, false>(a, p, s) : launch_fast<T, D, false, false>(a, p, s);
   const int st = a.mask ? launch_fast<T, D, true, true>(a, p, s) : launch_fast<T, D, false, true>(a, p, s);
   if (st != KESSIE_OK) return st;
-  const int64_t rows = (int64_t)a.B * a.max_q * a.Hq;
-  hipLaunchKernelGGL((cross_combine_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  if (p.waves) {
+    hipLaunchKernelGGL((cross_merge_kernel<T, D>), dim3((unsigned)(p.tiles * a.Hkv), div_up(p.part_rows, 1024 / D)), dim3(256), 0, s, a,
+                       p.waves * 32, 64);
+    return check_launch("cross attention (merge)");
+  }
+  int heads = 256 / D;  // (a wave's at once)
+  while (heads < a.Hq && (int64_t)a.Tq * div_up(a.Hq, heads) > 16 * attn::device_cus()) heads *= 2;
+  hipLaunchKernelGGL((cross_combine_kernel<T, D>), dim3(div_up(a.Tq, 4), div_up(a.Hq, heads)), dim3(256), 0, s, a, 32,
+                     rows_waves<T, D>() * kRowsKeys, heads);
   return check_launch("cross attention (combine)");
-}
-
-size_t partial_bytes(const Plan& p, int Tq, int Hq, int D) {
-  return p.S > 1 ? (size_t)Tq * Hq * p.S * (D + 2) * sizeof(float) : 0;
 }
 
 template <typename T>
@@ -879,19 +1238,20 @@ int launch(Args& a, void* ws, size_t ws_bytes, hipStream_t s) {
                     // (a tile's bytes within a buffer's 31 bits)
                     a.k_ts >= 0 && a.v_ts >= 0 && a.k_ts * (int64_t)sizeof(T) < (1 << 24) && a.v_ts * (int64_t)sizeof(T) < (1 << 24);
   if (!fast) return launch_generic<T>(a, s);
-  const Plan p = make_plan(a.B, a.max_q, a.Tq, a.Hq, a.Hkv, a.D, a.max_kv, (int)sizeof(T));
-  KESSIE_REQUIRE(p.tiles * a.Hkv * (p.few ? p.S : 1) <= 0x7fffffff && (int64_t)a.B * a.max_q * a.Hq <= (int64_t)4 * 0x7fffffff,
-                 KESSIE_ERR_UNSUPPORTED, "cross attention: %d sequences of up to %d queries exceed one launch", a.B, a.max_q);
-  const size_t need = partial_bytes(p, a.Tq, a.Hq, a.D);
-  KESSIE_REQUIRE(ws_bytes >= need && (need == 0 || (ws && aligned16(ws))), KESSIE_ERR_WORKSPACE,
-                 "cross attention: workspace of %zu bytes, %zu needed", ws_bytes, need);
-  a.S = p.S;
-  if (need) {
-    a.ws_o = static_cast<float*>(ws);
-    a.ws_m = a.ws_o + (size_t)a.Tq * a.Hq * p.S * a.D;
-    a.ws_l = a.ws_m + (size_t)a.Tq * a.Hq * p.S;
+  const Plan p = make_plan(a.B, a.max_q, a.Tq, a.Hq, a.Hkv, a.D, a.max_kv, a.Tkv, (int)sizeof(T));
+  KESSIE_REQUIRE(p.grid * a.Hkv <= 0x7fffffff, KESSIE_ERR_UNSUPPORTED,
+                 "cross attention: %d sequences of up to %d queries exceed one launch", a.B, a.max_q);
+  const Layout l = layout(p, a.B, a.Hkv, a.D);
+  KESSIE_REQUIRE(ws_bytes >= l.bytes && (l.bytes == 0 || (ws && aligned16(ws))), KESSIE_ERR_WORKSPACE,
+                 "cross attention: workspace of %zu bytes, %zu needed", ws_bytes, l.bytes);
+  if (l.bytes) {
+    a.shares = p.shares, a.min_steps = p.min_steps, a.part_rows = p.part_rows;
+    a.plan = static_cast<int64_t*>(ws);
+    a.ws_o = reinterpret_cast<float*>(static_cast<char*>(ws) + l.plan);
+    a.ws_m = a.ws_o + l.rows * a.D;
+    a.ws_l = a.ws_m + l.rows;
   }
-  return a.D == 64 ? launch_split<T, 64>(a, p, s) : launch_split<T, 128>(a, p, s);
+  return a.D == 64 ? launch_shared<T, 64>(a, p, s) : launch_shared<T, 128>(a, p, s);
 }
 
 }  // namespace
@@ -901,13 +1261,14 @@ int launch(Args& a, void* ws, size_t ws_bytes, hipStream_t s) {
 using namespace kessie;
 using namespace kessie::cross;
 
-extern "C" size_t kessie_cross_attention_workspace_bytes(int batch, int max_query_len, int num_q_tokens, int num_q_heads,
-                                                         int num_kv_heads, int head_dim, int max_kv_len, int dtype) {
-  if (batch <= 0 || max_query_len <= 0 || num_q_tokens <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || max_kv_len < 0 ||
+extern "C" size_t kessie_cross_attention_workspace_bytes(int batch, int max_query_len, int num_q_tokens, int num_kv_tokens,
+                                                         int num_q_heads, int num_kv_heads, int head_dim, int max_kv_len,
+                                                         int dtype) {
+  if (batch <= 0 || max_query_len <= 0 || num_q_tokens <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || max_kv_len < 0 || num_kv_tokens < 0 ||
       (head_dim != 64 && head_dim != 128))
     return 0;
-  return partial_bytes(make_plan(batch, max_query_len, num_q_tokens, num_q_heads, num_kv_heads, head_dim, max_kv_len, dtype_size(dtype)),
-                       num_q_tokens, num_q_heads, head_dim);
+  const Plan p = make_plan(batch, max_query_len, num_q_tokens, num_q_heads, num_kv_heads, head_dim, max_kv_len, num_kv_tokens, dtype_size(dtype));
+  return layout(p, batch, num_kv_heads, head_dim).bytes;
 }
 
 extern "C" int kessie_cross_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k,

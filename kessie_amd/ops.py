@@ -671,7 +671,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_sta
     lib = _lib.load()
     with _on(dev):
         if ws is None:
-            ws = workspace(lib.kessie_cross_attention_workspace_bytes(b, mq, t, hq, hkv, d, mk, dt), dev, "cross")
+            ws = workspace(lib.kessie_cross_attention_workspace_bytes(b, mq, t, n, hq, hkv, d, mk, dt), dev, "cross")
         _lib.check("kessie_cross_attention", lib.kessie_cross_attention(
             _ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1),
             _ptr(_contig(query_start_loc, "query_start_loc")), _ptr(_contig(kv_start, "kv_start")),

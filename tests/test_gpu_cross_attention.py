@@ -268,7 +268,7 @@ def test_streams_and_own_workspaces(dev, seqs):
     a, b = case(dev, seqs, 32, 8, 128, torch.bfloat16, seed=1), case(dev, seqs, 32, 8, 128, torch.bfloat16, seed=2)
     want = [attend(a), attend(b)]
     t = a["q"].shape[0]
-    need = _lib.load().kessie_cross_attention_workspace_bytes(len(seqs), seqs[0][0], t, 32, 8, 128, seqs[0][1], _lib.DTYPE_BF16)
+    need = _lib.load().kessie_cross_attention_workspace_bytes(len(seqs), seqs[0][0], t, a["k"].shape[0], 32, 8, 128, seqs[0][1], _lib.DTYPE_BF16)
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
     wss = [torch.empty(max(need, 1), dtype=torch.uint8, device=dev) for _ in streams]
     outs = [torch.zeros_like(a["q"]) for _ in streams]
@@ -284,7 +284,7 @@ def test_streams_and_own_workspaces(dev, seqs):
 def test_a_workspace_that_is_too_small_is_refused(dev):
     from kessie_amd import _lib
     c = case(dev, [(1, 60000)], 8, 1, 128, torch.bfloat16, seed=1)
-    need = _lib.load().kessie_cross_attention_workspace_bytes(1, 1, c["q"].shape[0], 8, 1, 128, 60000, _lib.DTYPE_BF16)
+    need = _lib.load().kessie_cross_attention_workspace_bytes(1, 1, c["q"].shape[0], 60000, 8, 1, 128, 60000, _lib.DTYPE_BF16)
     if need:
         out = torch.full_like(c["q"], FILL)
         with pytest.raises(_lib.KeSSieError) as e:
