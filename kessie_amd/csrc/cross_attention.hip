@@ -496,17 +496,13 @@ template <bool kMerge>
 __device__ __forceinline__ bool find_piece(const Args& a, int x, int rows, int keys, int& limit, int lane, Piece& p) {
   Seq mine = lane_sequence(a, 0, lane);
   if (limit < 0) {
-    float work = 0.0f, tiles = 0.0f;  // (fp32: every workgroup comes to the same limit, exact or not)
+    float work = 0.0f;  // (fp32: every workgroup comes to the same limit, exact or not)
     for (int b0 = 0; b0 < a.B; b0 += 64) {
       if (b0 > 0) mine = lane_sequence(a, b0, lane);
-      float n = (float)row_tiles(a, mine, rows), w = n * (float)steps_of(mine, keys);
+      float w = (float)row_tiles(a, mine, rows) * (float)steps_of(mine, keys);
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) {
-        w += __shfl_xor(w, o, 64);
-        n += __shfl_xor(n, o, 64);
-      }
+      for (int o = 32; o > 0; o >>= 1) w += __shfl_xor(w, o, 64);
       work += w;
-      tiles += n;
     }
     if (a.B > 64) mine = lane_sequence(a, 0, lane);
     // (ceil, and a little more for what the sums were rounded off: at most `shares` pieces and one a row tile.)
@@ -934,35 +930,27 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   }
 }
 
-// Merges the pieces of 1024 / D rows of a row tile, in order, eight loads in flight.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void cross_merge_kernel(Args a, int rows_per, int keys) {
-  constexpr int kLanes = D / 4, kRows = 256 / kLanes, kAhead = 8;
-  const int lane = threadIdx.x & 63, d = 4 * (threadIdx.x % kLanes);
-  const int g = blockIdx.x % a.Hkv;
-  Piece p;
-  int limit = uniform(*reinterpret_cast<const int32_t*>(a.plan));
-  if (!find_piece<true>(a, blockIdx.x / a.Hkv, rows_per, keys, limit, lane, p) || p.pieces == 1) return;
-  const int rows = min(p.sq.nq * a.G - p.rt * rows_per, rows_per), r = blockIdx.y * kRows + threadIdx.x / kLanes;
-  if (r >= rows) return;
-  const int64_t at = ((int64_t)p.first * a.Hkv + g) * a.part_rows + r, step = (int64_t)a.Hkv * a.part_rows;
-  // The online form: a piece's maximum and sum with its values.
+// Sums n partials of a row, the i-th at row at(i) of the workspace, elements d ..
+// d + 3: in order, by maximum and sum (the online form), eight in flight.
+template <int D, typename F>
+__device__ __forceinline__ f32x4 merge_partials(const Args& a, int n, int d, F at) {
+  constexpr int kAhead = 8;
   float top = kNegInf, sum = 0.0f;
   f32x4 y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int i0 = 0; i0 < p.pieces; i0 += kAhead) {
+  for (int i0 = 0; i0 < n; i0 += kAhead) {
     float m[kAhead], l[kAhead];
     f32x4 v[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int64_t n = at + (int64_t)min(i0 + i, p.pieces - 1) * step;
-      m[i] = a.ws_m[n];
-      l[i] = a.ws_l[n];
-      v[i] = *reinterpret_cast<const f32x4*>(a.ws_o + n * D + d);
+      const int64_t row = at(min(i0 + i, n - 1));
+      m[i] = a.ws_m[row];
+      l[i] = a.ws_l[row];
+      v[i] = *reinterpret_cast<const f32x4*>(a.ws_o + row * D + d);
     }
     float mn = top;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      if (i0 + i >= p.pieces) m[i] = kNegInf;
+      if (i0 + i >= n) m[i] = kNegInf;
       mn = fmaxf(mn, m[i]);
     }
     const float use = mn == kNegInf ? 0.0f : mn, was = __builtin_amdgcn_exp2f(top - use);
@@ -978,13 +966,33 @@ __global__ __launch_bounds__(256) void cross_merge_kernel(Args a, int rows_per, 
       }
     }
   }
-  const float il = sum != 0.0f ? 1.0f / sum : 0.0f;
-  const int row = p.rt * rows_per + r, pos = (unsigned)row / (unsigned)a.G, h = g * a.G + row - pos * a.G;
+  return y * (sum != 0.0f ? 1.0f / sum : 0.0f);
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* to, f32x4 y) {
   typedef T V __attribute__((ext_vector_type(4)));
   V z;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) z[k] = from_f32<T>(y[k] * il);
-  *reinterpret_cast<V*>(static_cast<T*>(a.out) + (int64_t)(p.sq.q0 + pos) * a.o_ts + (int64_t)h * a.o_hs + d) = z;
+  for (int k = 0; k < 4; ++k) z[k] = from_f32<T>(y[k]);
+  *reinterpret_cast<V*>(to) = z;
+}
+
+// Merges the pieces of `rows_wg` rows of a row tile.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cross_merge_kernel(Args a, int rows_per, int keys, int rows_wg) {
+  constexpr int kLanes = D / 4, kAtOnce = 256 / kLanes;
+  const int lane = threadIdx.x & 63, d = 4 * (threadIdx.x % kLanes);
+  const int g = blockIdx.x % a.Hkv;
+  Piece p;
+  int limit = uniform(*reinterpret_cast<const int32_t*>(a.plan));
+  if (!find_piece<true>(a, blockIdx.x / a.Hkv, rows_per, keys, limit, lane, p) || p.pieces == 1) return;
+  const int rows = min(p.sq.nq * a.G - p.rt * rows_per, rows_per), end = min((int)(blockIdx.y + 1) * rows_wg, rows);
+  const int64_t step = (int64_t)a.Hkv * a.part_rows, at = ((int64_t)p.first * a.Hkv + g) * a.part_rows;
+  for (int r = blockIdx.y * rows_wg + threadIdx.x / kLanes; r < end; r += kAtOnce) {
+    const f32x4 y = merge_partials<D>(a, p.pieces, d, [&](int i) { return at + r + i * step; });
+    const int row = p.rt * rows_per + r, pos = (unsigned)row / (unsigned)a.G, h = g * a.G + row - pos * a.G;
+    store4(static_cast<T*>(a.out) + (int64_t)(p.sq.q0 + pos) * a.o_ts + (int64_t)h * a.o_hs + d, y);
+  }
 }
 
 // Merges the partials of rows that several workgroups share, in step order.  One
@@ -1025,26 +1033,8 @@ __global__ __launch_bounds__(256) void cross_combine_kernel(Args a, int rows_per
     }
     if (j0 == j1 || h0 + sub >= h_end) continue;  // stored already
     // Partial of workgroup j: number 1 of the first, 0 of those after it.
-    auto part = [&](int j) { return (((int64_t)j * a.Hkv + g) * 2 + (j == j0)) * a.part_rows + r; };
-    float top = kNegInf;
-    for (int j = j0; j <= j1; ++j) top = fmaxf(top, a.ws_m[part(j)]);
-    const float use = top == kNegInf ? 0.0f : top;
-    f32x4 y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float sum = 0.0f;
-#pragma unroll 4
-    for (int j = j0; j <= j1; ++j) {
-      const int64_t p = part(j);
-      const float e = __builtin_amdgcn_exp2f(a.ws_m[p] - use);
-      const f32x4 v = *reinterpret_cast<const f32x4*>(a.ws_o + p * D + d);
-      sum += e * a.ws_l[p];
-      if (e != 0.0f) y += e * v;
-    }
-    const float il = sum != 0.0f ? 1.0f / sum : 0.0f;
-    typedef T V __attribute__((ext_vector_type(4)));
-    V z;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) z[k] = from_f32<T>(y[k] * il);
-    *reinterpret_cast<V*>(static_cast<T*>(a.out) + (int64_t)t * a.o_ts + (int64_t)h * a.o_hs + d) = z;
+    const f32x4 y = merge_partials<D>(a, j1 - j0 + 1, d, [&](int i) { return (((int64_t)(j0 + i) * a.Hkv + g) * 2 + (i == 0)) * a.part_rows + r; });
+    store4(static_cast<T*>(a.out) + (int64_t)t * a.o_ts + (int64_t)h * a.o_hs + d, y);
   }
 }
 
@@ -1163,7 +1153,8 @@ Plan make_plan(int B, int max_q, int Tq, int Hq, int Hkv, int D, int max_kv, int
   } else {
     // Eight waves share a tile's load where that still gives every CU a workgroup: 4,096 queries on 16,384 (32 / 8
     // heads of 128) 931 us against 1,015 with four; 8 x 200 on 1,000 (8 heads) 32.2 against 23.9.
-    p.waves = es == 2 && tiles_of(256) * Hkv >= cus ? 8 : 4;
+    // Shorter sequences fill tiles of 256 rows less well.
+    p.waves = es == 2 && tiles_of(256) * Hkv >= cus && (int64_t)Tq * G >= (int64_t)1024 * B ? 8 : 4;
     const int rows = p.waves * 32;
     p.tiles = tiles_of(rows);
     p.part_rows = (int)(most < rows ? most : rows);
@@ -1176,7 +1167,7 @@ Plan make_plan(int B, int max_q, int Tq, int Hq, int Hkv, int D, int max_kv, int
   // Split where the longest sequence would outlast an even share of the work by more than the merge costs (`gain`
   // steps: 5 us of it in decoding, 10 otherwise).  What an even share is goes by the means that the host knows.
   const int64_t slots = (int64_t)cus * per_cu;
-  const double mean = B > 0 && Tkv / B < max_kv ? (double)Tkv / B : max_kv, tiles = (double)Tq * G / (p.waves ? p.waves * 32 : 32) + 0.5 * B;
+  const double mean = B > 0 && Tkv / B < max_kv ? (double)Tkv / B : max_kv, tiles = p.waves ? (double)Tq * G / (p.waves * 32) + 0.5 * B : B;
   const double even = (tiles < p.tiles ? tiles : (double)p.tiles) * Hkv * (mean / keys + 0.5) / (double)slots;
   if (div_up(max_kv, keys) - even >= gain) {
     p.shares = (int)((slots + Hkv - 1) / Hkv);
@@ -1218,8 +1209,10 @@ int launch_shared(const Args& a, const Plan& p, hipStream_t s) {
   const int st = a.mask ? launch_fast<T, D, true, true>(a, p, s) : launch_fast<T, D, false, true>(a, p, s);
   if (st != KESSIE_OK) return st;
   if (p.waves) {
-    hipLaunchKernelGGL((cross_merge_kernel<T, D>), dim3((unsigned)(p.tiles * a.Hkv), div_up(p.part_rows, 1024 / D)), dim3(256), 0, s, a,
-                       p.waves * 32, 64);
+    // 32 rows a workgroup, fewer where that leaves the device idle (each finds its row tile first).
+    const int rows_wg = p.tiles * a.Hkv * div_up(p.part_rows, 32) < 2 * attn::device_cus() ? 1024 / D : 32;
+    hipLaunchKernelGGL((cross_merge_kernel<T, D>), dim3((unsigned)(p.tiles * a.Hkv), div_up(p.part_rows, rows_wg)), dim3(256), 0, s, a,
+                       p.waves * 32, 64, rows_wg);
     return check_launch("cross attention (merge)");
   }
   int heads = 256 / D;  // (a wave's at once)

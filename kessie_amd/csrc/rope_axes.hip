@@ -14,7 +14,7 @@
 // Three uses of one body: Q and K into tensors (or in place), Q into a tensor
 // with K and V into their cache slots, and K in place in its pages by the
 // difference of two positions.  Bound: HBM -- each row read and written once,
-// with 16-byte loads that are asked for before the angles are computed.
+// with 16-byte loads that are under way while the angles are computed.
 #include "common.h"
 
 namespace kessie {
@@ -49,6 +49,8 @@ struct Args {
   const float* inv;
   uint64_t axis[kMaxHalf / 32];  // two bits a pair
   int T, Hq, Hk, Hv, D, half;
+  int page_shift;    // page_size = 1 << page_shift, or -1
+  float inv_heads, inv_half;  // 1 / (Hq + Hk + Hv), 1 / half
   float sign;  // -1: rotate back
 };
 
@@ -75,16 +77,25 @@ __device__ __forceinline__ int axis_of(const Args& a, int j) {
   return (int)(w >> (2 * (j & 31))) & 3;
 }
 
-__device__ __forceinline__ double pos_at(const void* p, int64_t i, int is64) {
-  return is64 ? (double)static_cast<const int64_t*>(p)[i] : (double)static_cast<const int32_t*>(p)[i];
-}
-
-// (cos, sin) of token t's pair j.
-__device__ __forceinline__ float2 turn(const Args& a, int t, int j) {
+// What token t's pair j turns by, as loaded: without a branch, so that the loads
+// are under way together with the rows' (each is 4 bytes; a position of 32 bits
+// is loaded twice).
+struct Turn {
+  int lo, hi, from_lo, from_hi;
+  float inv;
+};
+__device__ __forceinline__ Turn load_turn(const Args& a, int t, int j) {
   const int ax = axis_of(a, j);
-  double p = pos_at(a.pos, ax * a.pos_as + t, a.pos64);
-  if (a.from) p -= pos_at(a.from, ax * a.from_as + t, a.pos64);
-  const double r = p * (double)a.inv[j] * 0.15915494309189533577;  // turns
+  const int width = a.pos64 ? 2 : 1, more = a.pos64 ? 1 : 0;
+  const int32_t* p = static_cast<const int32_t*>(a.pos) + (ax * a.pos_as + t) * width;
+  const int32_t* f = static_cast<const int32_t*>(a.from ? a.from : a.pos) + (ax * (a.from ? a.from_as : a.pos_as) + t) * width;
+  return {p[0], p[more], f[0], f[more], a.inv[j]};
+}
+// (cos, sin): the turns in 64 bits, their fraction in 32.
+__device__ __forceinline__ float2 angle(const Args& a, const Turn& u) {
+  auto whole = [&](int lo, int hi) { return (int64_t)(((uint64_t)(uint32_t)(a.pos64 ? hi : lo >> 31) << 32) | (uint32_t)lo); };
+  const int64_t p = whole(u.lo, u.hi) - (a.from ? whole(u.from_lo, u.from_hi) : 0);
+  const double r = (double)p * (double)u.inv * 0.15915494309189533577;
   float s, c;
   sincospif(2.0f * (float)(r - rint(r)), &s, &c);
   return make_float2(c, s * a.sign);
@@ -97,10 +108,10 @@ __device__ __forceinline__ int64_t pool_row(const Args& a, int t) {
   if (a.slots) {
     const int64_t slot = a.slots[t];
     if (slot < 0) return -1;
-    page = slot / a.page_size;
+    page = a.page_shift >= 0 ? slot >> a.page_shift : slot / a.page_size;
     off = (int)(slot - page * a.page_size);
   } else {
-    const int i = t / a.page_size;
+    const int i = a.page_shift >= 0 ? t >> a.page_shift : t / a.page_size;
     page = a.pages[i];
     off = t - i * a.page_size;
   }
@@ -108,34 +119,35 @@ __device__ __forceinline__ int64_t pool_row(const Args& a, int t) {
   return page * a.page_stride + off * a.tok_stride;
 }
 
-// Where head h of token t comes from and goes to (h counts Q's, K's and V's heads); false: nowhere.
+// Where head h of token t (h counts Q's, K's and V's heads) comes from; K in place in the pages: nullptr.
 template <typename T>
-__device__ __forceinline__ bool row_of(const Args& a, int t, int h, int64_t prow, const T*& src, T*& dst, bool& rot) {
+__device__ __forceinline__ const T* source(const Args& a, int t, int h, bool& rot) {
   rot = true;
-  if (h < a.Hq) {
-    src = static_cast<const T*>(a.q) + t * a.q_ts + h * a.q_hs;
-    dst = static_cast<T*>(a.qo) + t * a.qo_ts + h * a.qo_hs;
-    return true;
-  }
+  if (h < a.Hq) return static_cast<const T*>(a.q) + t * a.q_ts + h * a.q_hs;
   h -= a.Hq;
-  if (a.pool && prow < 0) return false;
-  if (h < a.Hk) {
-    dst = a.pool ? static_cast<T*>(a.pool) + prow + h * a.head_stride : static_cast<T*>(a.ko) + t * a.ko_ts + h * a.ko_hs;
-    src = a.k ? static_cast<const T*>(a.k) + t * a.k_ts + h * a.k_hs : dst;  // (no k: in place in the pages)
-    return true;
-  }
-  h -= a.Hk;
+  if (h < a.Hk) return a.k ? static_cast<const T*>(a.k) + t * a.k_ts + h * a.k_hs : nullptr;
   rot = false;
-  src = static_cast<const T*>(a.v) + t * a.v_ts + h * a.v_hs;
-  dst = static_cast<T*>(a.pool) + prow + h * a.head_stride + a.kv_stride;
-  return true;
+  return static_cast<const T*>(a.v) + t * a.v_ts + (h - a.Hk) * a.v_hs;
+}
+// And where it goes, or nullptr: nowhere.
+template <typename T>
+__device__ __forceinline__ T* target(const Args& a, int t, int h) {
+  if (h < a.Hq) return static_cast<T*>(a.qo) + t * a.qo_ts + h * a.qo_hs;
+  h -= a.Hq;
+  if (!a.pool) return static_cast<T*>(a.ko) + t * a.ko_ts + h * a.ko_hs;
+  const int64_t row = pool_row(a, t);
+  if (row < 0) return nullptr;
+  return static_cast<T*>(a.pool) + row + (h < a.Hk ? h * a.head_stride : (h - a.Hk) * a.head_stride + a.kv_stride);
 }
 
 // 16-byte chunks, two a thread and step: chunk pair i of a row holds both
 // halves of N pairs (or, adjacent, two neighbouring chunks), and past the
 // rotated part two chunks to copy, so every row is D / 2N steps of the same
-// kind.  kTok tokens a workgroup.
-template <typename T, bool kAdjacent, int kThreads, int kTok, int kSteps>
+// kind.  kTok tokens a workgroup.  kPer fixes D / 2N (0: any), kPages a K that
+// is rotated in place in its pages: the index arithmetic before the first load
+// is then shifts (with the angles' loads ahead of the rows', 89 -> 77 us at
+// 65,536 tokens).
+template <typename T, bool kAdjacent, bool kPages, int kPer, int kThreads, int kTok, int kSteps>
 __global__ __launch_bounds__(kThreads) void rope_axes_vec(Args a) {
   typedef typename Vec16<T>::type V;
   constexpr int N = Vec16<T>::N;
@@ -143,13 +155,20 @@ __global__ __launch_bounds__(kThreads) void rope_axes_vec(Args a) {
   const int half = a.half, R = 2 * half;
   const int t0 = blockIdx.x * kTok;
   const int ntok = min(kTok, a.T - t0);
-  const int heads = a.Hq + a.Hk + a.Hv;
-  const int per = a.D / (2 * N);                 // steps a row
-  const int stride = kThreads / per;             // rows a round
+  const int heads = kPages ? a.Hk : a.Hq + a.Hk + a.Hv;
+  const int per = kPer > 0 ? kPer : a.D / (2 * N);  // steps a row
+  const int stride = kThreads / per;                // rows a round
   const int i = threadIdx.x % per, r0 = threadIdx.x / per;
   const int o1 = kAdjacent ? 2 * i * N : i * N < half ? i * N : i * N + half;
   const int o2 = kAdjacent ? o1 + N : i * N < half ? o1 + half : o1 + (a.D - R) / 2;
   const int rows = r0 < stride ? ntok * heads : 0;
+  // This thread's first angle is asked for before the rows: its wait is then not theirs too.
+  auto angle_at = [&](int n) {
+    const int tt = (int)(((float)n + 0.5f) * a.inv_half);
+    return load_turn(a, t0 + tt, n - tt * half);
+  };
+  const int angles = ntok * half;
+  const Turn first = angle_at(min((int)threadIdx.x, angles - 1));
   bool ready = false;
   for (int base = r0;; base += kSteps * stride) {
     V x1[kSteps], x2[kSteps];
@@ -161,26 +180,30 @@ __global__ __launch_bounds__(kThreads) void rope_axes_vec(Args a) {
       dst[s] = nullptr;
       csi[s] = -1;
       if (row < rows) {
-        const int tt = kTok == 1 ? 0 : kTok == 2 ? (row >= heads ? 1 : 0) : row / heads;
+        // (exact: row + 1/2 is at least 1/2 from a multiple of heads, and both are small)
+        const int tt = kTok == 1 ? 0 : kTok == 2 ? (row >= heads ? 1 : 0) : (int)(((float)row + 0.5f) * a.inv_heads);
         const int h = row - tt * heads;
         const T* src;
-        T* to;
-        bool rot;
-        if (row_of<T>(a, t0 + tt, h, a.pool && h >= a.Hq ? pool_row(a, t0 + tt) : 0, src, to, rot)) {
-          if (rot) csi[s] = tt * half;
-          if (src != to || o1 < R) {  // (in place, the rest of the row stays)
-            dst[s] = to;
-            x1[s] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src + o1));
-            x2[s] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src + o2));
-          }
+        bool rot = true;
+        if constexpr (kPages) {
+          const int64_t at = pool_row(a, t0 + tt);
+          dst[s] = at < 0 || o1 >= R ? nullptr : static_cast<T*>(a.pool) + at + h * a.head_stride;
+          src = dst[s];
+        } else {
+          src = source<T>(a, t0 + tt, h, rot);
+          dst[s] = target<T>(a, t0 + tt, h);
+          if (src == dst[s] && o1 >= R) dst[s] = nullptr;  // (in place, the rest of the row stays)
+        }
+        if (rot) csi[s] = tt * half;
+        if (src) {
+          x1[s] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src + o1));
+          x2[s] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src + o2));
         }
       }
     }
     if (!ready) {
-      for (int n = threadIdx.x; n < ntok * half; n += kThreads) {
-        const int tt = n / half;
-        cs[n] = turn(a, t0 + tt, n - tt * half);
-      }
+      if (threadIdx.x < angles) cs[threadIdx.x] = angle(a, first);
+      for (int n = threadIdx.x + kThreads; n < angles; n += kThreads) cs[n] = angle(a, angle_at(n));
       __syncthreads();
       ready = true;
     }
@@ -232,10 +255,11 @@ __global__ __launch_bounds__(256) void rope_axes_scalar(Args a) {
     const int i = (int)(n % per);
     const int64_t th = n / per;
     const int t = (int)(th / heads), h = (int)(th - (int64_t)t * heads);
-    const T* src;
-    T* dst;
     bool rot;
-    if (!row_of<T>(a, t, h, a.pool && h >= a.Hq ? pool_row(a, t) : 0, src, dst, rot)) continue;
+    const T* src = source<T>(a, t, h, rot);
+    T* dst = target<T>(a, t, h);
+    if (dst == nullptr) continue;
+    if (src == nullptr) src = dst;
     if (i >= a.half) {
       const int d = R + i - a.half;
       if (src != dst) dst[d] = src[d];
@@ -247,7 +271,7 @@ __global__ __launch_bounds__(256) void rope_axes_scalar(Args a) {
       dst[d2] = src[d2];
       continue;
     }
-    const float2 w = turn(a, t, i);
+    const float2 w = angle(a, load_turn(a, t, i));
     const float u = to_f32(src[d1]), z = to_f32(src[d2]);
     dst[d1] = from_f32<T>(fmaf(u, w.x, -(z * w.y)));
     dst[d2] = from_f32<T>(fmaf(u, w.y, z * w.x));
@@ -268,10 +292,22 @@ int launch(const Args& a, hipStream_t s) {
     const int64_t items = (int64_t)a.T * heads * (a.half + a.D - R);
     const int64_t grid = (items + 255) / 256;
     hipLaunchKernelGGL((rope_axes_scalar<T, kAdjacent>), dim3((unsigned)(grid < (1 << 20) ? grid : 1 << 20)), dim3(256), 0, s, a);
-  } else if (a.k == nullptr && a.Hq == 0) {  // in place in the pages
-    hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, 1024, 16, 1>), dim3(div_up(a.T, 16)), dim3(1024), 0, s, a);
+  } else if (a.k == nullptr && a.Hq == 0) {
+    // In place in the pages: a page's 16 tokens a workgroup.  65,536 bf16 tokens of 8 heads x 128 in random interleaved
+    // pages (270 MB): 77.0 us, 8 tokens of 512 threads 80.4, 4 of 256 79.4, the tiles of a page on one XCD 77-79; with
+    // the pages in order 61-64, so what bounds it is where the pages lie.
+    if (per == 8)
+      hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, true, 8, 1024, 16, 1>), dim3(div_up(a.T, 16)), dim3(1024), 0, s, a);
+    else
+      hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, true, 0, 512, 8, 1>), dim3(div_up(a.T, 8)), dim3(512), 0, s, a);
+  } else if (per == 8) {
+    // 16,411 bf16 tokens, 32 + 8 + 8 heads of 128, K and V to their slots (404 MB): 70.1 us = 5.8 TB/s; 256 threads 72.2.
+    hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, false, 8, 512, 2, 2>), dim3(div_up(a.T, 2)), dim3(512), 0, s, a);
+  } else if (per == 4) {
+    // 9,005 fp16 tokens, 16 + 16 heads of 64 (74 MB): 17.2 us; 4 tokens 18.4, 1 token 17.6.
+    hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, false, 4, 256, 2, 1>), dim3(div_up(a.T, 2)), dim3(256), 0, s, a);
   } else {
-    hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, 256, 2, 3>), dim3(div_up(a.T, 2)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, false, 0, 256, 2, 3>), dim3(div_up(a.T, 2)), dim3(256), 0, s, a);
   }
   return check_launch("rope axes");
 }
@@ -313,6 +349,9 @@ int dispatch(Args& a, const int32_t* sections, int num_axes, int interleaved, in
     a.axis[j >> 5] |= (uint64_t)use << (2 * (j & 31));
   }
   a.sign = inverse ? -1.0f : 1.0f;
+  a.page_shift = a.page_size > 0 && (a.page_size & (a.page_size - 1)) == 0 ? __builtin_ctz((unsigned)a.page_size) : -1;
+  a.inv_heads = 1.0f / (float)(a.Hq + a.Hk + a.Hv > 0 ? a.Hq + a.Hk + a.Hv : 1);
+  a.inv_half = 1.0f / (float)a.half;
   if (a.T == 0 || a.Hq + a.Hk == 0) return KESSIE_OK;
   KESSIE_REQUIRE(a.pos && a.inv, KESSIE_ERR_INVALID, "rope axes: null pointer");
   switch (dtype) {

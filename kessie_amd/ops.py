@@ -434,18 +434,36 @@ def rope_remap_paged(pool: torch.Tensor, orig_pos: torch.Tensor, tgt_pos: torch.
 # ---------------------------------------------------------------------------
 # Rotary positions with several axes
 # ---------------------------------------------------------------------------
-def _one_device(dev: torch.device, **tensors: Optional[torch.Tensor]) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, not on {dev}")
+def _gpu_index(t: torch.Tensor, name: str) -> int:
+    i = t.get_device()
+    if i < 0:
+        raise ValueError(f"{name} must be on the GPU, got {t.device}")
+    return i
+
+
+def _one_device(dev: int, *named) -> None:
+    """Every (name, tensor or None) of ``named`` on GPU ``dev``: a kernel is handed plain addresses."""
+    for name, t in named:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name} is on {t.device}, not on cuda:{dev}")
 
 
 _here = contextlib.nullcontext()
 
 
-def _on(dev: torch.device):
-    """The device a launch belongs to made current (nothing to do where it is already)."""
-    return _here if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _on(dev: int):
+    """GPU ``dev`` made current for a launch (nothing to do where it is already)."""
+    return _here if torch.cuda.current_device() == dev else torch.cuda.device(dev)
+
+
+def _raw_stream(stream, dev: int) -> int:
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(dev)
+    return _stream_ptr(stream, dev).value or 0
+
+
+def _addr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 _sections: dict = {}
@@ -526,14 +544,14 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
         raise ValueError("k_out without k")
     row = _positions_arg(positions, len(sections), t, "positions")
     r = _inv_arg(inv_freq, d)
-    dev = q.device
-    _one_device(dev, k=k, q_out=q_out, k_out=k_out, positions=positions, inv_freq=inv_freq)
+    dev = _gpu_index(q, "q")
+    _one_device(dev, ("k", k), ("q_out", q_out), ("k_out", k_out), ("positions", positions), ("inv_freq", inv_freq))
+    (qs0, qs1, _), (qo0, qo1, _) = q.stride(), q_out.stride()
     with _on(dev):
         _lib.check("kessie_rope_axes", _lib.load().kessie_rope_axes(
-            _ptr(q), q.stride(0), q.stride(1), _ptr(q_out), q_out.stride(0), q_out.stride(1), hq, _ptr(k), ks0, ks1,
-            _ptr(k_out), os0, os1, hkv, _ptr(positions), row, positions.dtype == torch.int64, _ptr(inv_freq),
-            _sections_arg(sections), len(sections), interleaved, adjacent, inverse, t, d, r, dtype_code(q.dtype),
-            _stream_ptr(stream, dev)))
+            q.data_ptr(), qs0, qs1, q_out.data_ptr(), qo0, qo1, hq, _addr(k), ks0, ks1, _addr(k_out), os0, os1, hkv,
+            positions.data_ptr(), row, positions.dtype == torch.int64, inv_freq.data_ptr(), _sections_arg(sections),
+            len(sections), interleaved, adjacent, inverse, t, d, r, dtype_code(q.dtype), _raw_stream(stream, dev)))
     return q_out, k_out
 
 
@@ -567,15 +585,17 @@ def rope_axes_cache_write(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.T
         raise ValueError("slot_mapping must be int64 with one entry per token")
     row = _positions_arg(positions, len(sections), t, "positions")
     r = _inv_arg(inv_freq, d)
-    dev = pool.device
-    _one_device(dev, q=q, q_out=q_out, k=k, v=v, positions=positions, slot_mapping=slot_mapping, inv_freq=inv_freq)
+    dev = _gpu_index(pool, "pool")
+    _one_device(dev, ("q", q), ("q_out", q_out), ("k", k), ("v", v), ("positions", positions), ("slot_mapping", slot_mapping),
+                ("inv_freq", inv_freq))
+    _contig(slot_mapping, "slot_mapping")
+    (ks0, ks1, _), (vs0, vs1, _) = k.stride(), v.stride()
     with _on(dev):
         _lib.check("kessie_rope_axes_cache_write", _lib.load().kessie_rope_axes_cache_write(
-            _ptr(q), qs0, qs1, _ptr(q_out), os0, os1, hq, _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0),
-            v.stride(1), h, _ptr(positions), row, positions.dtype == torch.int64, _ptr(inv_freq),
-            _sections_arg(sections), len(sections), interleaved, adjacent, C.c_void_p(pv.k_ptr), pv.page_stride,
-            pv.tok_stride, pv.kv_stride, pv.head_stride, _ptr(_contig(slot_mapping, "slot_mapping")), pv.page_size,
-            pv.num_pages, t, d, r, dtype_code(k.dtype), _stream_ptr(stream, dev)))
+            _addr(q), qs0, qs1, _addr(q_out), os0, os1, hq, k.data_ptr(), ks0, ks1, v.data_ptr(), vs0, vs1, h,
+            positions.data_ptr(), row, positions.dtype == torch.int64, inv_freq.data_ptr(), _sections_arg(sections),
+            len(sections), interleaved, adjacent, pv.k_ptr, pv.page_stride, pv.tok_stride, pv.kv_stride, pv.head_stride,
+            slot_mapping.data_ptr(), pv.page_size, pv.num_pages, t, d, r, dtype_code(k.dtype), _raw_stream(stream, dev)))
     return q_out
 
 
@@ -595,23 +615,23 @@ def rope_remap_axes(pool: torch.Tensor, orig_pos: torch.Tensor, tgt_pos: torch.T
     if page_list is None:
         _rows3(pool, "k", (t,) + tuple(pool.shape[1:]))
         _, h, d = pool.shape
-        ptr, ps, (ts, hs, _), n_pages, p_size = _ptr(pool), 0, pool.stride(), 0, 0
+        ptr, ps, (ts, hs, _), n_pages, p_size = pool.data_ptr(), 0, pool.stride(), 0, 0
     else:
         pv = pool_view(pool, layout)
         if page_list.dtype != torch.int32 or not page_list.is_contiguous():
             raise TypeError("page_list must be contiguous int32")
         if page_list.numel() * pv.page_size < t:
             raise ValueError("page_list too short for the token count")
-        ptr, ps, ts, hs = C.c_void_p(pv.k_ptr), pv.page_stride, pv.tok_stride, pv.head_stride
+        ptr, ps, ts, hs = pv.k_ptr, pv.page_stride, pv.tok_stride, pv.head_stride
         n_pages, p_size, h, d = pv.num_pages, pv.page_size, pv.num_kv_heads, pv.head_dim
     r = _inv_arg(inv_freq, d)
-    dev = pool.device
-    _one_device(dev, orig_pos=orig_pos, tgt_pos=tgt_pos, inv_freq=inv_freq, page_list=page_list)
+    dev = _gpu_index(pool, "pool")
+    _one_device(dev, ("orig_pos", orig_pos), ("tgt_pos", tgt_pos), ("inv_freq", inv_freq), ("page_list", page_list))
     with _on(dev):
         _lib.check("kessie_rope_remap_axes", _lib.load().kessie_rope_remap_axes(
-            ptr, ps, ts, hs, _ptr(page_list), n_pages, _ptr(orig_pos), r0, _ptr(tgt_pos), r1,
-            orig_pos.dtype == torch.int64, _ptr(inv_freq), _sections_arg(sections), axes, interleaved, adjacent, t, h, d,
-            r, p_size, dtype_code(pool.dtype), _stream_ptr(stream, dev)))
+            ptr, ps, ts, hs, _addr(page_list), n_pages, orig_pos.data_ptr(), r0, tgt_pos.data_ptr(), r1,
+            orig_pos.dtype == torch.int64, inv_freq.data_ptr(), _sections_arg(sections), axes, interleaved, adjacent, t, h,
+            d, r, p_size, dtype_code(pool.dtype), _raw_stream(stream, dev)))
 
 
 # ---------------------------------------------------------------------------
@@ -661,23 +681,25 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_sta
         out = torch.empty(t, hq, d, dtype=q.dtype, device=q.device)
     else:
         _rows3(out, "out", q.shape, q.dtype)
-    dev = q.device
-    _one_device(dev, k=k, v=v, query_start_loc=query_start_loc, kv_start=kv_start, kv_lens=kv_lens, key_mask=key_mask,
-                out=out, ws=ws)
+    dev = _gpu_index(q, "q")
+    _one_device(dev, ("k", k), ("v", v), ("query_start_loc", query_start_loc), ("kv_start", kv_start), ("kv_lens", kv_lens),
+                ("key_mask", key_mask), ("out", out), ("ws", ws))
+    if not (query_start_loc.is_contiguous() and kv_start.is_contiguous() and kv_lens.is_contiguous()):
+        raise ValueError("query_start_loc, kv_start and kv_lens must be contiguous")
     dt = dtype_code(q.dtype)
     mq, mk = min(int(max_query_len), t), min(int(max_kv_len), n)
     if sm_scale is None:
         sm_scale = d ** -0.5
     lib = _lib.load()
+    (qs0, qs1, _), (ks0, ks1, _), (vs0, vs1, _), (os0, os1, _) = q.stride(), k.stride(), v.stride(), out.stride()
     with _on(dev):
         if ws is None:
-            ws = workspace(lib.kessie_cross_attention_workspace_bytes(b, mq, t, n, hq, hkv, d, mk, dt), dev, "cross")
+            need = lib.kessie_cross_attention_workspace_bytes(b, mq, t, n, hq, hkv, d, mk, dt)
+            ws = workspace(need, q.device, "cross") if need else None
         _lib.check("kessie_cross_attention", lib.kessie_cross_attention(
-            _ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1),
-            _ptr(_contig(query_start_loc, "query_start_loc")), _ptr(_contig(kv_start, "kv_start")),
-            _ptr(_contig(kv_lens, "kv_lens")), _ptr(key_mask), _ptr(out), out.stride(0), out.stride(1), b, mq, mk, t, n,
-            hq, hkv, d, float(sm_scale), dt, _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size(),
-            _stream_ptr(stream, dev)))
+            q.data_ptr(), qs0, qs1, k.data_ptr(), ks0, ks1, v.data_ptr(), vs0, vs1, query_start_loc.data_ptr(),
+            kv_start.data_ptr(), kv_lens.data_ptr(), _addr(key_mask), out.data_ptr(), os0, os1, b, mq, mk, t, n, hq, hkv, d,
+            float(sm_scale), dt, _addr(ws), 0 if ws is None else ws.numel() * ws.element_size(), _raw_stream(stream, dev)))
     return out
 
 
@@ -690,6 +712,9 @@ class StepTables(NamedTuple):
     slot_mapping: torch.Tensor     # int64 [rows]
     positions: torch.Tensor        # int32 [rows]
     taken: torch.Tensor            # int32 [1]
+
+
+_STEP_DTYPES = (torch.int32, torch.int32, torch.int64, torch.int32, torch.int32)
 
 
 def step_tables(block_table: torch.Tensor, computed_lens: torch.Tensor, new_lens: torch.Tensor, page_size: int,
@@ -739,30 +764,30 @@ def step_tables(block_table: torch.Tensor, computed_lens: torch.Tensor, new_lens
         if page_valid is not None and page_positions.numel() != num_pages:
             raise ValueError("page_valid and page_positions differ in length")
         num_pages = page_positions.numel()
-    dev = block_table.device
     if out is None:
+        dev = block_table.device
         ints = torch.empty(2 * b + 2 + num_token_rows, dtype=torch.int32, device=dev)
         out = StepTables(ints[:b + 1], ints[b + 1:2 * b + 1], torch.empty(num_token_rows, dtype=torch.int64, device=dev),
                          ints[2 * b + 2:], ints[2 * b + 1:2 * b + 2])
     else:
         out = out if type(out) is StepTables else StepTables(*out)
-        for name, t, dt, n in zip(StepTables._fields, out, (torch.int32, torch.int32, torch.int64, torch.int32, torch.int32),
-                                  (b + 1, b, num_token_rows, num_token_rows, 1)):
+        for name, t, dt, n in zip(StepTables._fields, out, _STEP_DTYPES, (b + 1, b, num_token_rows, num_token_rows, 1)):
             if t.dtype != dt or t.numel() != n or not t.is_contiguous():
                 raise ValueError(f"out.{name} must be a contiguous {dt} tensor of {n} entries")
-    _one_device(dev, computed_lens=computed_lens, new_lens=new_lens, free_pages=free_pages, free_count=free_count,
-                position_delta=position_delta, page_valid=page_valid, page_positions=page_positions, **out._asdict())
-    for name, t in (("computed_lens", computed_lens), ("new_lens", new_lens), ("free_pages", free_pages),
-                    ("position_delta", position_delta), ("page_valid", page_valid), ("page_positions", page_positions)):
-        if t is not None:
-            _contig(t, name)
+    dev = _gpu_index(block_table, "block_table")
+    given = (("computed_lens", computed_lens), ("new_lens", new_lens), ("free_pages", free_pages),
+             ("position_delta", position_delta), ("page_valid", page_valid), ("page_positions", page_positions))
+    for name, t in given:
+        if t is not None and not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    _one_device(dev, *given, ("free_count", free_count), *zip(StepTables._fields, out))
+    rows, width = block_table.shape
     with _on(dev):
         _lib.check("kessie_step_tables", _lib.load().kessie_step_tables(
-            _ptr(block_table), block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1],
-            block_table.shape[1], _ptr(computed_lens), _ptr(new_lens),
-            _ptr(position_delta), _ptr(free_pages) if max_free else None, _ptr(free_count), max_free, b, int(page_size),
-            int(num_token_rows), _ptr(out[0]), _ptr(out[1]), _ptr(out[2]), _ptr(out[3]), _ptr(out[4]), _ptr(page_valid),
-            _ptr(page_positions), num_pages, _stream_ptr(stream, dev)))
+            block_table.data_ptr(), block_table.stride(0) if rows > 1 else width, width, computed_lens.data_ptr(),
+            new_lens.data_ptr(), _addr(position_delta), _addr(free_pages), _addr(free_count), max_free, b, int(page_size),
+            int(num_token_rows), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(),
+            out[4].data_ptr(), _addr(page_valid), _addr(page_positions), num_pages, _raw_stream(stream, dev)))
     return out
 
 
