@@ -565,8 +565,8 @@ __device__ __forceinline__ void store_row(T* row, const f32x16 (&o)[D / 32], flo
     }
 }
 
-// Up to 32 rows of a (sequence, kv head): decoding.  A step is NW tiles, one a
-// wave; every wave streams its tiles through two LDS stages of its own, the next
+// 32 rows of a (sequence, kv head): decoding, and prompts too small to fill the
+// device with larger tiles.  A step is NW tiles, one a wave; every wave streams its tiles through two LDS stages of its own, the next
 // tile in flight while one is computed: no barrier before the merge.  Bound: HBM.
 template <typename T, int D, int KT, int NW, bool kMask, bool kShare>
 __global__ __launch_bounds__(NW * 64) void cross_rows_kernel(Args a) {
@@ -587,9 +587,9 @@ __global__ __launch_bounds__(NW * 64) void cross_rows_kernel(Args a) {
   do {
   const Stretch now = uniform(walk.now);
   const Seq sq = now.sq;
-  const int rows = sq.nq * a.G;
+  const int row0 = now.rt * 32, rows = min(sq.nq * a.G - row0, 32);
   typename C::QV q[C::QN];
-  C::load_q(a, sq, min(col, rows - 1), g, half, q, col < rows);
+  C::load_q(a, sq, row0 + min(col, rows - 1), g, half, q, col < rows);
   const char* kbase = static_cast<const char*>(a.k) + ((int64_t)sq.kv0 * a.k_ts + (int64_t)g * a.k_hs) * (int64_t)sizeof(T);
   const char* vbase = static_cast<const char*>(a.v) + ((int64_t)sq.kv0 * a.v_ts + (int64_t)g * a.v_hs) * (int64_t)sizeof(T);
   const int nkv = (int)min((int64_t)sq.nkv, (int64_t)now.end * (NW * KT));  // states up to this stretch's end
@@ -689,7 +689,7 @@ __global__ __launch_bounds__(NW * 64) void cross_rows_kernel(Args a) {
       sum += e * sl[w * 32 + r];
       if (e != 0.0f) y += e * *reinterpret_cast<const f32x4*>(so + (w * 32 + r) * kOut + d);
     }
-    const int pos = (unsigned)r / (unsigned)a.G, h = g * a.G + r - pos * a.G;
+    const int pos = (unsigned)(row0 + r) / (unsigned)a.G, h = g * a.G + row0 + r - pos * a.G;
     if (kShare && !(now.t == 0 && now.end == now.steps)) {
       const int64_t row = part_row(a, now.t == 0, r);
       *reinterpret_cast<f32x4*>(a.ws_o + row * D + d) = y;
@@ -1142,14 +1142,18 @@ Plan make_plan(int B, int max_q, int Tq, int Hq, int Hkv, int D, int max_kv, int
   };
   Plan p{};
   int keys, per_cu, gain;
-  if (most <= 32) {
-    const int nw = row_bytes == 512 ? 2 : 4;
-    p.tiles = B;
-    p.part_rows = (int)most;
+  const int nw = row_bytes == 512 ? 2 : 4, rows_per_cu = 160 * 1024 / (nw * 4 * kRowsKeys * row_bytes);
+  // Few rows altogether over few states (at most three tiles a wave): the waves of a workgroup share the states of 32
+  // rows and merge them in LDS.  1 x 40 on 300 (fp32, 8 heads of 64) 15.2 us against 18.5 with 128 rows a workgroup;
+  // past that it loses: 8 x 60 on 1,000 (bf16, 8 heads of 128) 19.9 against 17.1.
+  const bool small = tiles_of(32) * Hkv <= (int64_t)cus * rows_per_cu && max_kv <= 3 * nw * kRowsKeys;
+  if (most <= 32 || small) {
+    p.tiles = most <= 32 ? B : tiles_of(32);
+    p.part_rows = (int)(most < 32 ? most : 32);
     p.min_steps = 2;
     keys = nw * kRowsKeys;
-    per_cu = 160 * 1024 / (nw * 4 * kRowsKeys * row_bytes);
-    gain = 5;
+    per_cu = rows_per_cu;
+    gain = most <= 32 ? 5 : 1 << 30;
   } else {
     // Eight waves share a tile's load where that still gives every CU a workgroup: 4,096 queries on 16,384 (32 / 8
     // heads of 128) 931 us against 1,015 with four; 8 x 200 on 1,000 (8 heads) 32.2 against 23.9.
