@@ -120,27 +120,32 @@ class PoolView:
         return self.base.data_ptr()
 
 
-def pool_view(pool: torch.Tensor, layout: str = "native") -> PoolView:
+def _pool_axes(pool: torch.Tensor, layout: str):
+    """(pages, page size, kv heads, head_dim, page / token / kv / head strides) of a pool."""
     if pool.dim() != 5:
         raise ValueError(f"pool must be 5-D, got shape {tuple(pool.shape)}")
-    s = pool.stride()
-    if s[4] != 1:
+    s0, s1, s2, s3, s4 = pool.stride()
+    if s4 != 1:
         raise ValueError("pool head_dim axis must be contiguous")
     if layout == "native":
         n, p, two, h, d = pool.shape
-        ps, ts, kvs, hs = s[0], s[1], s[2], s[3]
+        got = n, p, h, d, s0, s1, s2, s3
     elif layout == "kv_first":
         two, n, p, h, d = pool.shape
-        kvs, ps, ts, hs = s[0], s[1], s[2], s[3]
+        got = n, p, h, d, s1, s2, s0, s3
     elif layout == "block_kv":
         n, two, p, h, d = pool.shape
-        ps, kvs, ts, hs = s[0], s[1], s[2], s[3]
+        got = n, p, h, d, s0, s2, s1, s3
     else:
         raise ValueError(f"unknown pool layout {layout!r}")
     if two != 2:
         raise ValueError(f"pool K/V axis must have size 2, got {two}")
+    return got
+
+
+def pool_view(pool: torch.Tensor, layout: str = "native") -> PoolView:
     # Storage-offset-aware base: element [0,...] of K.
-    return PoolView(pool, n, p, h, d, ps, ts, kvs, hs)
+    return PoolView(pool, *_pool_axes(pool, layout))
 
 
 # ---------------------------------------------------------------------------
@@ -434,18 +439,15 @@ def rope_remap_paged(pool: torch.Tensor, orig_pos: torch.Tensor, tgt_pos: torch.
 # ---------------------------------------------------------------------------
 # Rotary positions with several axes
 # ---------------------------------------------------------------------------
-def _gpu_index(t: torch.Tensor, name: str) -> int:
-    i = t.get_device()
-    if i < 0:
-        raise ValueError(f"{name} must be on the GPU, got {t.device}")
-    return i
-
-
-def _one_device(dev: int, *named) -> None:
-    """Every (name, tensor or None) of ``named`` on GPU ``dev``: a kernel is handed plain addresses."""
-    for name, t in named:
+def _gpu(first: str, **tensors: Optional[torch.Tensor]) -> int:
+    """The GPU that ``tensors[first]`` is on; all others given must be there too (a kernel is handed plain addresses)."""
+    dev = tensors[first].get_device()
+    if dev < 0:
+        raise ValueError(f"{first} must be on the GPU, got {tensors[first].device}")
+    for name, t in tensors.items():
         if t is not None and t.get_device() != dev:
             raise ValueError(f"{name} is on {t.device}, not on cuda:{dev}")
+    return dev
 
 
 _here = contextlib.nullcontext()
@@ -544,8 +546,7 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
         raise ValueError("k_out without k")
     row = _positions_arg(positions, len(sections), t, "positions")
     r = _inv_arg(inv_freq, d)
-    dev = _gpu_index(q, "q")
-    _one_device(dev, ("k", k), ("q_out", q_out), ("k_out", k_out), ("positions", positions), ("inv_freq", inv_freq))
+    dev = _gpu("q", q=q, k=k, q_out=q_out, k_out=k_out, positions=positions, inv_freq=inv_freq)
     (qs0, qs1, _), (qo0, qo1, _) = q.stride(), q_out.stride()
     with _on(dev):
         _lib.check("kessie_rope_axes", _lib.load().kessie_rope_axes(
@@ -563,10 +564,10 @@ def rope_axes_cache_write(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.T
     in place or into q_out, rotated k and v [T, Hkv, D] written to the paged
     pool at slot_mapping[t] (int64, negative: not written).  k and v stay as
     they are.  Returns q_out."""
-    pv = pool_view(pool, layout)
+    pages, p, ph, pd, ps, ts, kvs, hs = _pool_axes(pool, layout)
     _rows3(k, "k")
     t, h, d = k.shape
-    if h != pv.num_kv_heads or d != pv.head_dim:
+    if h != ph or d != pd:
         raise ValueError("k/v heads or head_dim do not match the pool")
     if k.dtype != pool.dtype:
         raise TypeError("k/v dtype must match the pool")
@@ -585,17 +586,16 @@ def rope_axes_cache_write(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.T
         raise ValueError("slot_mapping must be int64 with one entry per token")
     row = _positions_arg(positions, len(sections), t, "positions")
     r = _inv_arg(inv_freq, d)
-    dev = _gpu_index(pool, "pool")
-    _one_device(dev, ("q", q), ("q_out", q_out), ("k", k), ("v", v), ("positions", positions), ("slot_mapping", slot_mapping),
-                ("inv_freq", inv_freq))
+    dev = _gpu("pool", pool=pool, q=q, q_out=q_out, k=k, v=v, positions=positions, slot_mapping=slot_mapping,
+               inv_freq=inv_freq)
     _contig(slot_mapping, "slot_mapping")
     (ks0, ks1, _), (vs0, vs1, _) = k.stride(), v.stride()
     with _on(dev):
         _lib.check("kessie_rope_axes_cache_write", _lib.load().kessie_rope_axes_cache_write(
             _addr(q), qs0, qs1, _addr(q_out), os0, os1, hq, k.data_ptr(), ks0, ks1, v.data_ptr(), vs0, vs1, h,
             positions.data_ptr(), row, positions.dtype == torch.int64, inv_freq.data_ptr(), _sections_arg(sections),
-            len(sections), interleaved, adjacent, pv.k_ptr, pv.page_stride, pv.tok_stride, pv.kv_stride, pv.head_stride,
-            slot_mapping.data_ptr(), pv.page_size, pv.num_pages, t, d, r, dtype_code(k.dtype), _raw_stream(stream, dev)))
+            len(sections), interleaved, adjacent, pool.data_ptr(), ps, ts, kvs, hs, slot_mapping.data_ptr(), p, pages, t, d, r,
+            dtype_code(k.dtype), _raw_stream(stream, dev)))
     return q_out
 
 
@@ -615,21 +615,18 @@ def rope_remap_axes(pool: torch.Tensor, orig_pos: torch.Tensor, tgt_pos: torch.T
     if page_list is None:
         _rows3(pool, "k", (t,) + tuple(pool.shape[1:]))
         _, h, d = pool.shape
-        ptr, ps, (ts, hs, _), n_pages, p_size = pool.data_ptr(), 0, pool.stride(), 0, 0
+        ps, (ts, hs, _), n_pages, p_size = 0, pool.stride(), 0, 0
     else:
-        pv = pool_view(pool, layout)
+        n_pages, p_size, h, d, ps, ts, _, hs = _pool_axes(pool, layout)
         if page_list.dtype != torch.int32 or not page_list.is_contiguous():
             raise TypeError("page_list must be contiguous int32")
-        if page_list.numel() * pv.page_size < t:
+        if page_list.numel() * p_size < t:
             raise ValueError("page_list too short for the token count")
-        ptr, ps, ts, hs = pv.k_ptr, pv.page_stride, pv.tok_stride, pv.head_stride
-        n_pages, p_size, h, d = pv.num_pages, pv.page_size, pv.num_kv_heads, pv.head_dim
     r = _inv_arg(inv_freq, d)
-    dev = _gpu_index(pool, "pool")
-    _one_device(dev, ("orig_pos", orig_pos), ("tgt_pos", tgt_pos), ("inv_freq", inv_freq), ("page_list", page_list))
+    dev = _gpu("pool", pool=pool, orig_pos=orig_pos, tgt_pos=tgt_pos, inv_freq=inv_freq, page_list=page_list)
     with _on(dev):
         _lib.check("kessie_rope_remap_axes", _lib.load().kessie_rope_remap_axes(
-            ptr, ps, ts, hs, _addr(page_list), n_pages, orig_pos.data_ptr(), r0, tgt_pos.data_ptr(), r1,
+            pool.data_ptr(), ps, ts, hs, _addr(page_list), n_pages, orig_pos.data_ptr(), r0, tgt_pos.data_ptr(), r1,
             orig_pos.dtype == torch.int64, inv_freq.data_ptr(), _sections_arg(sections), axes, interleaved, adjacent, t, h,
             d, r, p_size, dtype_code(pool.dtype), _raw_stream(stream, dev)))
 
@@ -681,9 +678,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_sta
         out = torch.empty(t, hq, d, dtype=q.dtype, device=q.device)
     else:
         _rows3(out, "out", q.shape, q.dtype)
-    dev = _gpu_index(q, "q")
-    _one_device(dev, ("k", k), ("v", v), ("query_start_loc", query_start_loc), ("kv_start", kv_start), ("kv_lens", kv_lens),
-                ("key_mask", key_mask), ("out", out), ("ws", ws))
+    dev = _gpu("q", q=q, k=k, v=v, query_start_loc=query_start_loc, kv_start=kv_start, kv_lens=kv_lens, key_mask=key_mask,
+               out=out, ws=ws)
     if not (query_start_loc.is_contiguous() and kv_start.is_contiguous() and kv_lens.is_contiguous()):
         raise ValueError("query_start_loc, kv_start and kv_lens must be contiguous")
     dt = dtype_code(q.dtype)
@@ -713,8 +709,6 @@ class StepTables(NamedTuple):
     positions: torch.Tensor        # int32 [rows]
     taken: torch.Tensor            # int32 [1]
 
-
-_STEP_DTYPES = (torch.int32, torch.int32, torch.int64, torch.int32, torch.int32)
 
 
 def step_tables(block_table: torch.Tensor, computed_lens: torch.Tensor, new_lens: torch.Tensor, page_size: int,
@@ -771,16 +765,22 @@ def step_tables(block_table: torch.Tensor, computed_lens: torch.Tensor, new_lens
                          ints[2 * b + 2:], ints[2 * b + 1:2 * b + 2])
     else:
         out = out if type(out) is StepTables else StepTables(*out)
-        for name, t, dt, n in zip(StepTables._fields, out, _STEP_DTYPES, (b + 1, b, num_token_rows, num_token_rows, 1)):
-            if t.dtype != dt or t.numel() != n or not t.is_contiguous():
-                raise ValueError(f"out.{name} must be a contiguous {dt} tensor of {n} entries")
-    dev = _gpu_index(block_table, "block_table")
-    given = (("computed_lens", computed_lens), ("new_lens", new_lens), ("free_pages", free_pages),
-             ("position_delta", position_delta), ("page_valid", page_valid), ("page_positions", page_positions))
-    for name, t in given:
+        starts, lens, slots, pos, taken = out
+        if not (starts.numel() == b + 1 and lens.numel() == b and slots.numel() == pos.numel() == num_token_rows
+                and taken.numel() == 1 and slots.dtype == torch.int64
+                and starts.dtype == lens.dtype == pos.dtype == taken.dtype == torch.int32 and starts.is_contiguous()
+                and lens.is_contiguous() and slots.is_contiguous() and pos.is_contiguous()):
+            raise ValueError(f"out must be contiguous int32 [{b + 1}], int32 [{b}], int64 [{num_token_rows}], int32 "
+                             f"[{num_token_rows}], int32 [1], got {[(x.dtype, tuple(x.shape)) for x in out]}")
+    dev = _gpu("block_table", block_table=block_table, computed_lens=computed_lens, new_lens=new_lens, free_pages=free_pages,
+               free_count=free_count, position_delta=position_delta, page_valid=page_valid, page_positions=page_positions,
+               query_start_loc=out[0], seq_lens=out[1], slot_mapping=out[2], positions=out[3], taken=out[4])
+    if not (computed_lens.is_contiguous() and new_lens.is_contiguous()):
+        raise ValueError("computed_lens and new_lens must be contiguous")
+    for name, t in (("free_pages", free_pages), ("position_delta", position_delta), ("page_valid", page_valid),
+                    ("page_positions", page_positions)):
         if t is not None and not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
-    _one_device(dev, *given, ("free_count", free_count), *zip(StepTables._fields, out))
     rows, width = block_table.shape
     with _on(dev):
         _lib.check("kessie_step_tables", _lib.load().kessie_step_tables(
