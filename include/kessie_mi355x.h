@@ -327,8 +327,8 @@ int kessie_rope_remap_paged(void* kv_pool, int64_t page_stride,
  * position for all axes).  inv_freq: fp32 [rotary_dim/2] on the device.  The
  * product pos * inv_freq is exact, not rounded to fp32.  Element (t, h, d) of
  * q lies at t*q_tok_stride + h*q_head_stride + d; outputs may be the inputs
- * (in place, same strides).  q or k may be NULL (with its output).
- * rotary_dim <= 256. */
+ * (in place, same strides); rows of an output may not overlap.  q or k may be
+ * NULL (with its output).  rotary_dim <= 256. */
 int kessie_rope_axes(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
                      void* q_out, int64_t q_out_tok_stride,
                      int64_t q_out_head_stride, int num_q_heads, const void* k,
@@ -345,7 +345,8 @@ int kessie_rope_axes(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
  * the rotated Q (may be q; q and q_out may both be NULL), the pool the rotated
  * K and the V of token t at slot_mapping[t] (int64; page = slot / page_size,
  * as kessie_kv_cache_write; rows of negative slots and of pages outside
- * [0, num_pages) are not written).  k and v themselves stay as they are. */
+ * [0, num_pages) are not written; no slot may occur twice).  k and v themselves
+ * stay as they are. */
 int kessie_rope_axes_cache_write(
     const void* q, int64_t q_tok_stride, int64_t q_head_stride, void* q_out,
     int64_t q_out_tok_stride, int64_t q_out_head_stride, int num_q_heads,
@@ -398,7 +399,9 @@ size_t kessie_cross_attention_workspace_bytes(int batch, int max_query_len,
  * k / v, zero hides that state; what k and v hold there is not used, be it NaN.  A
  * query that sees no state gives a zero row.  Rows of out past the last
  * sequence are left as they are.  Element (t, h, d) of q at t*q_tok_stride +
- * h*q_head_stride + d, likewise k, v and out.  head_dim <= 256; sums in fp32. */
+ * h*q_head_stride + d, likewise k, v and out (whose rows may not overlap).
+ * head_dim <= 256; sums in fp32.  The workspace is written by every call: calls
+ * that may overlap need one each. */
 int kessie_cross_attention(
     const void* q, int64_t q_tok_stride, int64_t q_head_stride, const void* k,
     int64_t k_tok_stride, int64_t k_head_stride, const void* v,
@@ -433,7 +436,8 @@ int kessie_cross_attention(
  *                       bits; 0 past the last token
  *   taken               int32 [1]: pages taken, the first ones of free_pages
  *   page_valid (int8), page_positions (int32): 1 and the page's first position
- *                       for every page taken (either may be NULL; num_pages entries). */
+ *                       for every page taken (either may be NULL; num_pages entries).
+ * KESSIE_ERR_INVALID if an output lies over an input or another output. */
 int kessie_step_tables(int32_t* block_table, int64_t table_stride,
                        int table_width, const int32_t* computed_lens,
                        const int32_t* new_lens, const int32_t* position_delta,

@@ -80,4 +80,13 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 __host__ __device__ __forceinline__ int div_up(int a, int b) { return (a + b - 1) / b; }
 __host__ __device__ __forceinline__ int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Rows of d elements at t*ts + h*hs, t < n and h < m, none over another: heads within a token's rows, or tokens within a
+// head's.
+inline bool rows_apart(int64_t n, int64_t ts, int64_t m, int64_t hs, int64_t d) {
+  if (n <= 0 || m <= 0) return true;
+  if (n == 1) ts = m * (hs > d ? hs : d);
+  if (m == 1) hs = n * (ts > d ? ts : d);
+  return (hs >= d && ts >= (m - 1) * hs + d) || (ts >= d && hs >= (n - 1) * ts + d);
+}
+
 }  // namespace kessie

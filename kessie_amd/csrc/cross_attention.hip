@@ -950,7 +950,7 @@ __device__ __forceinline__ f32x4 merge_partials(const Args& a, int n, int d, F a
     float mn = top;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      if (i0 + i >= n) m[i] = kNegInf;
+      if (i0 + i >= n) m[i] = kNegInf, l[i] = 0.0f;
       mn = fmaxf(mn, m[i]);
     }
     const float use = mn == kNegInf ? 0.0f : mn, was = __builtin_amdgcn_exp2f(top - use);
@@ -960,7 +960,7 @@ __device__ __forceinline__ f32x4 merge_partials(const Args& a, int n, int d, F a
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const float e = __builtin_amdgcn_exp2f(m[i] - use);
-      if (e != 0.0f) {
+      if (l[i] != 0.0f) {  // (a row of NaN scores has no maximum, but a sum: NaN)
         sum += e * l[i];
         y += e * v[i];
       }
@@ -1066,9 +1066,8 @@ __global__ __launch_bounds__(64) void cross_generic_kernel(Args a) {
     float top = y;
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-    const float mn = fmaxf(m, top);
-    if (mn == kNegInf) continue;  // (uniform: nothing seen so far)
-    const float alpha = exp2f(m - mn), p = exp2f(y - mn);
+    const float mn = fmaxf(m, top), use = mn == kNegInf ? 0.0f : mn;
+    const float alpha = exp2f(m - use), p = exp2f(y - use);
     m = mn;
     float sum = p;
 #pragma unroll
@@ -1089,7 +1088,7 @@ __global__ __launch_bounds__(64) void cross_generic_kernel(Args a) {
     }
   }
   T* out = static_cast<T*>(a.out) + (int64_t)(s.q0 + i) * a.o_ts + (int64_t)h * a.o_hs;
-  const float il = l > 0.0f ? 1.0f / l : 0.0f;
+  const float il = l != 0.0f ? 1.0f / l : 0.0f;
   for (int e = 0; e < kMaxD / 64; ++e)
     if (lane + 64 * e < a.D) out[lane + 64 * e] = from_f32<T>(o[e] * il);
 }
@@ -1097,7 +1096,7 @@ __global__ __launch_bounds__(64) void cross_generic_kernel(Args a) {
 template <typename T>
 int launch_generic(const Args& a, hipStream_t s) {
   const int64_t rows = (int64_t)a.B * a.max_q;
-  KESSIE_REQUIRE(rows <= 0x7fffffff, KESSIE_ERR_UNSUPPORTED, "cross attention: %lld rows exceed one launch", (long long)rows);
+  KESSIE_REQUIRE(rows < 1 << 26, KESSIE_ERR_UNSUPPORTED, "cross attention: %lld rows exceed one launch", (long long)rows);
   hipLaunchKernelGGL(cross_generic_kernel<T>, dim3((unsigned)rows, a.Hq), dim3(64), 0, s, a);
   return check_launch("cross attention");
 }
@@ -1236,8 +1235,9 @@ int launch(Args& a, void* ws, size_t ws_bytes, hipStream_t s) {
                     a.k_ts >= 0 && a.v_ts >= 0 && a.k_ts * (int64_t)sizeof(T) < (1 << 24) && a.v_ts * (int64_t)sizeof(T) < (1 << 24);
   if (!fast) return launch_generic<T>(a, s);
   const Plan p = make_plan(a.B, a.max_q, a.Tq, a.Hq, a.Hkv, a.D, a.max_kv, a.Tkv, (int)sizeof(T));
-  KESSIE_REQUIRE(p.grid * a.Hkv <= 0x7fffffff, KESSIE_ERR_UNSUPPORTED,
-                 "cross attention: %d sequences of up to %d queries exceed one launch", a.B, a.max_q);
+  // (A launch counts its threads in 32 bits, 512 a workgroup at most; the kernels count rows in 31.)
+  KESSIE_REQUIRE(p.grid * a.Hkv < 1 << 23 && a.Tq <= 1 << 26 && (int64_t)a.Tq * a.G <= 1 << 30, KESSIE_ERR_UNSUPPORTED,
+                 "cross attention: %d sequences, %d queries of %d heads exceed one launch", a.B, a.Tq, a.Hq);
   const Layout l = layout(p, a.B, a.Hkv, a.D);
   KESSIE_REQUIRE(ws_bytes >= l.bytes && (l.bytes == 0 || (ws && aligned16(ws))), KESSIE_ERR_WORKSPACE,
                  "cross attention: workspace of %zu bytes, %zu needed", ws_bytes, l.bytes);
@@ -1261,8 +1261,8 @@ using namespace kessie::cross;
 extern "C" size_t kessie_cross_attention_workspace_bytes(int batch, int max_query_len, int num_q_tokens, int num_kv_tokens,
                                                          int num_q_heads, int num_kv_heads, int head_dim, int max_kv_len,
                                                          int dtype) {
-  if (batch <= 0 || max_query_len <= 0 || num_q_tokens <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || max_kv_len < 0 || num_kv_tokens < 0 ||
-      (head_dim != 64 && head_dim != 128))
+  if (batch <= 0 || max_query_len <= 0 || num_q_tokens <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || max_kv_len < 0 ||
+      num_kv_tokens < 0 || (head_dim != 64 && head_dim != 128) || dtype_size(dtype) <= 0)
     return 0;
   const Plan p = make_plan(batch, max_query_len, num_q_tokens, num_q_heads, num_kv_heads, head_dim, max_kv_len, num_kv_tokens, dtype_size(dtype));
   return layout(p, batch, num_kv_heads, head_dim).bytes;
@@ -1291,6 +1291,8 @@ extern "C" int kessie_cross_attention(const void* q, int64_t q_tok_stride, int64
   if (batch == 0 || max_query_len == 0 || num_q_tokens == 0) return KESSIE_OK;
   KESSIE_REQUIRE(q && out && query_start_loc && kv_start && kv_lens && (num_kv_tokens == 0 || (k && v)), KESSIE_ERR_INVALID,
                  "cross attention: null pointer");
+  KESSIE_REQUIRE(rows_apart(num_q_tokens, out_tok_stride, num_q_heads, out_head_stride, head_dim), KESSIE_ERR_INVALID,
+                 "cross attention: rows of out overlap (strides %lld, %lld)", (long long)out_tok_stride, (long long)out_head_stride);
   Args a{};
   a.q = q, a.q_ts = q_tok_stride, a.q_hs = q_head_stride;
   a.k = k, a.k_ts = k_tok_stride, a.k_hs = k_head_stride;

@@ -153,7 +153,9 @@ __global__ __launch_bounds__(kThreads) void rope_axes_vec(Args a) {
   constexpr int N = Vec16<T>::N;
   __shared__ float2 cs[kTok * kMaxHalf];
   const int half = a.half, R = 2 * half;
-  const int t0 = blockIdx.x * kTok;
+  const int64_t tile = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  if (tile * kTok >= a.T) return;
+  const int t0 = (int)tile * kTok;
   const int ntok = min(kTok, a.T - t0);
   const int heads = kPages ? a.Hk : a.Hq + a.Hk + a.Hv;
   const int per = kPer > 0 ? kPer : a.D / (2 * N);  // steps a row
@@ -288,6 +290,11 @@ int launch(const Args& a, hipStream_t s) {
                    fine(a.ko, a.ko_ts, a.ko_hs) && fine(a.v, a.v_ts, a.v_hs) && fine(a.pool, a.tok_stride, a.head_stride) &&
                    (a.pool == nullptr || (a.page_stride % N == 0 && a.kv_stride % N == 0));
   const int heads = a.Hq + a.Hk + a.Hv;
+  // (A launch's x dimension counts its threads in 32 bits.)
+  auto tiles = [&](int64_t tok) {
+    const int64_t n = div_up((int64_t)a.T, tok), x = n < 1 << 21 ? n : 1 << 21;
+    return dim3((unsigned)x, (unsigned)div_up(n, x));
+  };
   if (!vec) {
     const int64_t items = (int64_t)a.T * heads * (a.half + a.D - R);
     const int64_t grid = (items + 255) / 256;
@@ -297,17 +304,17 @@ int launch(const Args& a, hipStream_t s) {
     // pages (270 MB): 77.0 us, 8 tokens of 512 threads 80.4, 4 of 256 79.4, the tiles of a page on one XCD 77-79; with
     // the pages in order 61-64, so what bounds it is where the pages lie.
     if (per == 8)
-      hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, true, 8, 1024, 16, 1>), dim3(div_up(a.T, 16)), dim3(1024), 0, s, a);
+      hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, true, 8, 1024, 16, 1>), tiles(16), dim3(1024), 0, s, a);
     else
-      hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, true, 0, 512, 8, 1>), dim3(div_up(a.T, 8)), dim3(512), 0, s, a);
+      hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, true, 0, 512, 8, 1>), tiles(8), dim3(512), 0, s, a);
   } else if (per == 8) {
     // 16,411 bf16 tokens, 32 + 8 + 8 heads of 128, K and V to their slots (404 MB): 70.1 us = 5.8 TB/s; 256 threads 72.2.
-    hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, false, 8, 512, 2, 2>), dim3(div_up(a.T, 2)), dim3(512), 0, s, a);
+    hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, false, 8, 512, 2, 2>), tiles(2), dim3(512), 0, s, a);
   } else if (per == 4) {
     // 9,005 fp16 tokens, 16 + 16 heads of 64 (74 MB): 17.2 us; 4 tokens 18.4, 1 token 17.6.
-    hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, false, 4, 256, 2, 1>), dim3(div_up(a.T, 2)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, false, 4, 256, 2, 1>), tiles(2), dim3(256), 0, s, a);
   } else {
-    hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, false, 0, 256, 2, 3>), dim3(div_up(a.T, 2)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((rope_axes_vec<T, kAdjacent, false, 0, 256, 2, 3>), tiles(2), dim3(256), 0, s, a);
   }
   return check_launch("rope axes");
 }
@@ -353,6 +360,8 @@ int dispatch(Args& a, const int32_t* sections, int num_axes, int interleaved, in
   a.inv_heads = 1.0f / (float)(a.Hq + a.Hk + a.Hv > 0 ? a.Hq + a.Hk + a.Hv : 1);
   a.inv_half = 1.0f / (float)a.half;
   if (a.T == 0 || a.Hq + a.Hk == 0) return KESSIE_OK;
+  KESSIE_REQUIRE(rows_apart(a.T, a.qo_ts, a.Hq, a.qo_hs, a.D) && (a.pool || rows_apart(a.T, a.ko_ts, a.Hk, a.ko_hs, a.D)),
+                 KESSIE_ERR_INVALID, "rope axes: rows of an output overlap");
   KESSIE_REQUIRE(a.pos && a.inv, KESSIE_ERR_INVALID, "rope axes: null pointer");
   switch (dtype) {
     case KESSIE_DTYPE_BF16: return adjacent ? launch<bf16_t, true>(a, s) : launch<bf16_t, false>(a, s);
@@ -414,7 +423,7 @@ extern "C" int kessie_rope_axes_cache_write(
   KESSIE_REQUIRE(page_size > 0 && num_pages >= 0 && num_kv_heads > 0, KESSIE_ERR_INVALID, "rope axes: bad sizes P=%d pages=%d Hkv=%d",
                  page_size, num_pages, num_kv_heads);
   KESSIE_REQUIRE(num_tokens <= 0 || (k && v && kv_pool && slot_mapping), KESSIE_ERR_INVALID, "rope axes: null pointer");
-  KESSIE_REQUIRE(head_stride >= head_dim && tok_stride >= (int64_t)num_kv_heads * head_stride && kv_stride > 0, KESSIE_ERR_INVALID,
+  KESSIE_REQUIRE(rows_apart(page_size, tok_stride, num_kv_heads, head_stride, head_dim) && kv_stride > 0, KESSIE_ERR_INVALID,
                  "rope axes: pool strides overlap");
   return dispatch(a, sections, num_axes, interleaved, adjacent, 0, rotary_dim, dtype, as_stream(stream));
 }
@@ -431,11 +440,12 @@ extern "C" int kessie_rope_remap_axes(void* kv_pool, int64_t page_stride, int64_
   a.from = orig_pos, a.from_as = orig_axis_stride;
   a.inv = inv_freq;
   a.T = num_tokens, a.Hk = num_heads, a.D = head_dim;
-  KESSIE_REQUIRE(num_heads > 0 && head_stride >= head_dim && tok_stride >= (int64_t)num_heads * head_stride, KESSIE_ERR_INVALID,
-                 "rope axes: strides overlap (tok %lld head %lld)", (long long)tok_stride, (long long)head_stride);
+  KESSIE_REQUIRE(num_heads > 0, KESSIE_ERR_INVALID, "rope axes: %d heads", num_heads);
   KESSIE_REQUIRE(num_tokens <= 0 || (kv_pool && orig_pos), KESSIE_ERR_INVALID, "rope axes: null pointer");
   if (page_list) {
     KESSIE_REQUIRE(page_size > 0 && num_pages >= 0, KESSIE_ERR_INVALID, "rope axes: page_size=%d num_pages=%d", page_size, num_pages);
+    KESSIE_REQUIRE(rows_apart(page_size, tok_stride, num_heads, head_stride, head_dim), KESSIE_ERR_INVALID,
+                   "rope axes: pool strides overlap (tok %lld head %lld)", (long long)tok_stride, (long long)head_stride);
     a.pool = kv_pool, a.page_stride = page_stride, a.tok_stride = tok_stride, a.head_stride = head_stride;
     a.pages = page_list, a.page_size = page_size, a.num_pages = num_pages;
   } else {  // dense rows

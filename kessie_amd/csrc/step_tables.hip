@@ -229,6 +229,27 @@ extern "C" int kessie_step_tables(int32_t* block_table, int64_t table_stride, in
                  "step tables: a free list needs its pages and its count");
   KESSIE_REQUIRE(table_stride >= table_width, KESSIE_ERR_INVALID, "step tables: table rows overlap (stride %lld, width %d)",
                  (long long)table_stride, table_width);
+  // Every workgroup reads the lengths while others write the tables: none of these may lie over another.
+  struct Range {
+    const void* at;
+    int64_t bytes;
+  };
+  const int64_t B = batch, T = num_token_rows, W = batch ? (B - 1) * table_stride + table_width : 0;
+  const Range in[] = {{computed_lens, 4 * B}, {new_lens, 4 * B}, {position_delta, 4 * B}, {free_pages, 4 * (int64_t)max_free},
+                      {max_free ? free_count : nullptr, 4}};
+  const Range out[] = {{query_start_loc, 4 * B + 4}, {seq_lens, 4 * B}, {slot_mapping, 8 * T}, {positions, 4 * T}, {taken, 4},
+                       {block_table, 4 * W}, {page_valid, num_pages}, {page_positions, 4 * (int64_t)num_pages}};
+  constexpr int kOut = sizeof(out) / sizeof(out[0]);
+  auto over = [](const Range& x, const Range& y) {
+    const char *p = static_cast<const char*>(x.at), *q = static_cast<const char*>(y.at);
+    return p && q && x.bytes > 0 && y.bytes > 0 && p < q + y.bytes && q < p + x.bytes;
+  };
+  for (int i = 0; i < kOut; ++i) {
+    for (const Range& x : in)
+      KESSIE_REQUIRE(!over(x, out[i]), KESSIE_ERR_INVALID, "step tables: an input lies over an output");
+    for (int j = 0; j < i; ++j)
+      KESSIE_REQUIRE(!over(out[j], out[i]), KESSIE_ERR_INVALID, "step tables: two outputs lie over each other");
+  }
   Args a{block_table, table_stride, table_width, computed_lens, new_lens, position_delta,
          max_free ? free_pages : nullptr, free_count, max_free, batch, page_size, num_token_rows, query_start_loc,
          seq_lens, slot_mapping, positions, taken, page_valid, page_positions, num_pages};

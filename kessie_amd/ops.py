@@ -483,6 +483,8 @@ def _sections_arg(sections: Sequence[int]):
 
 def _positions_arg(p: torch.Tensor, axes: int, t: int, name: str) -> int:
     """The stride between the axes' rows of positions [axes, T], or 0 for [T]."""
+    if t >= 1 << 31:
+        raise ValueError(f"{t} tokens: fewer than 2^31 are taken")
     if p.dtype != torch.int32 and p.dtype != torch.int64:
         raise TypeError(f"{name} must be int32 or int64")
     if p.dim() == 1 and p.shape[0] == t:
@@ -729,7 +731,9 @@ def step_tables(block_table: torch.Tensor, computed_lens: torch.Tensor, new_lens
     page_valid (int8) and page_positions (int32), if given, are set to 1 and to
     the page's first position for the pages taken.
 
-    ``out``: a StepTables (or tuple of its five tensors) to fill again."""
+    ``out``: a StepTables (or tuple of its five tensors) to fill again.  No
+    output may share memory with an input: the last step's ``seq_lens`` are
+    this one's ``computed_lens`` as a copy, or with another ``out``."""
     if block_table.dtype != torch.int32 or computed_lens.dtype != torch.int32 or new_lens.dtype != torch.int32:
         raise TypeError("block_table, computed_lens and new_lens must be int32")
     b = computed_lens.numel()

@@ -185,6 +185,28 @@ def test_infinite_values_come_through(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("d", [64, 128, 80])
+@pytest.mark.parametrize("q,n", [(1, 60), (1, 9000), (40, 60), (200, 4000)])
+def test_nan_scores_come_through(dev, dtype, d, q, n):
+    """A row whose scores are all NaN is NaN, and the rows beside it are as they were, also where the states are split; so is
+    every row over a NaN key."""
+    c = case(dev, [(q, n), (q, 50)], 8, 2, d, dtype, seed=15)
+    want = attend(c)
+    c["q"][q // 2, 3] = float("nan")
+    got = attend(c)
+    assert got[q // 2, 3].isnan().all()
+    got[q // 2, 3] = want[q // 2, 3]
+    assert torch.equal(got, want)
+    c = case(dev, [(q, n), (q, 50)], 8, 2, d, dtype, seed=15)
+    c["k"] = c["k"].clone()
+    c["k"][n - 1, 1] = float("nan")
+    got = attend(c)
+    assert got[:q, 4:].isnan().all()
+    got[:q, 4:] = want[:q, 4:]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("q", [1, 40])
 def test_shared_overlapping_and_cut_ranges(dev, dtype, q):
     from kessie_amd import ops

@@ -209,6 +209,29 @@ def test_rows_that_are_not_16_byte_aligned(dev, offset):
     check(q, want)
 
 
+@pytest.mark.parametrize("t", [1, 37])
+def test_head_major_rows(dev, t):
+    """Tensors [H, T, D] seen as [T, H, D]: as inputs, outputs, and rotated in place."""
+    from kessie_amd import ops
+    pos, back, inv = positions(dev, 2, t, 5000, 1), positions(dev, 2, t, 5000, 2), inv_freq(32, 1e4, dev)
+    q = randn((6, t, 64), torch.float16, dev, 3).transpose(0, 1)
+    out = torch.zeros(6, t, 64, dtype=torch.float16, device=dev).transpose(0, 1)
+    ops.rope_axes(q, None, pos, inv, (16, 16), q_out=out)
+    check(out, rotate64(q, pos, inv, (16, 16)))
+    want = rotate64(out, back.long() - pos, inv, (16, 16))
+    ops.rope_remap_axes(out, pos, back, inv, (16, 16))
+    check(out, want)
+
+
+def test_more_tokens_than_one_grid_dimension(dev):
+    from kessie_amd import ops
+    t = (1 << 22) + 5
+    q, pos, inv = randn((t, 1, 16), torch.bfloat16, dev, 3), positions(dev, 2, t, 1_000_000, 1), inv_freq(8, 1e4, dev)
+    want = rotate64(q, pos, inv, (4, 4))
+    ops.rope_axes(q, None, pos, inv, (4, 4))
+    check(q, want)
+
+
 def test_large_rows_past_32_bit_offsets(dev):
     """Token rows whose elements lie past 2^31: 70,000 tokens 32,768 elements apart (a 4.3 GiB projection)."""
     from kessie_amd import ops

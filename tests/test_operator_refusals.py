@@ -122,3 +122,52 @@ def test_step_tables_refusals():
                 dict(computed_lens=[120, 0], new_lens=[9, 0]), dict(num_token_rows=1), dict(page_size=0), dict(position_delta=[1])):
         with pytest.raises(ValueError):
             Meta.build(**{**dict(block_table=i32(2, 8), computed_lens=[0, 0], new_lens=[1, 1], page_size=16, free_pages=i32(5)), **bad})
+
+
+def test_rows_of_an_output_that_overlap_are_refused():
+    """At the C entries, before any launch (the addresses are the host's)."""
+    from kessie_amd import _lib
+    lib = _lib.load()
+    buf = torch.zeros(64, dtype=torch.int64)
+    p, sec = buf.data_ptr(), (C.c_int32 * 1)(32)
+
+    def rope(ts, hs, t=5, hq=4):
+        return lib.kessie_rope_axes(p, 0, 0, p, ts, hs, hq, None, 0, 0, None, 0, 0, 0, None, 0, 0, None, sec, 1, 0, 0, 0, t, 64, 64, 1, None)
+
+    def remap(ts, hs, pages=None):
+        return lib.kessie_rope_remap_axes(p, 1 << 20, ts, hs, pages, 1, p, 0, None, 0, 0, None, sec, 1, 0, 0, 5, 4, 64, 64, 16, 1, None)
+
+    def cross(ts, hs):
+        return lib.kessie_cross_attention(p, 0, 0, p, 0, 0, p, 0, 0, p, p, p, None, p, ts, hs, 1, 5, 1, 5, 1, 4, 2, 64, 0.1, 1, None, 0, None)
+    for call in (rope, remap, lambda ts, hs: remap(ts, hs, p), cross):
+        for ts, hs in ((0, 64), (64, 0), (64, 64), (255, 64), (256, 63), (63, 64 * 5)):
+            assert call(ts, hs) != _lib.OK
+            assert "overlap" in _lib.last_error()[1], (ts, hs)
+        for ts, hs in ((256, 64), (64, 64 * 16), (1000, 65)) if call is not cross else ():  # (a null pointer ends those)
+            assert call(ts, hs) != _lib.OK and "overlap" not in _lib.last_error()[1], (ts, hs)
+    assert rope(0, 64, t=1) != _lib.OK and "overlap" not in _lib.last_error()[1]
+    assert rope(64, 0, hq=1) != _lib.OK and "overlap" not in _lib.last_error()[1]
+
+
+def test_workspace_of_an_unknown_type():
+    from kessie_amd import _lib
+    assert _lib.load().kessie_cross_attention_workspace_bytes(1, 1, 1, 60000, 8, 1, 64, 60000, 7) == 0
+
+
+def test_step_tables_that_lie_over_each_other_are_refused():
+    """In place (last step's seq_lens as computed_lens and out at once), and outputs that share memory: before any launch."""
+    from kessie_amd import _lib
+    lib = _lib.load()
+    names = ["table", "computed", "new", "delta", "free", "count", "starts", "lens", "slots", "pos", "taken", "valid", "where"]
+    own = {n: torch.zeros(64, dtype=torch.int64) for n in names}
+
+    def status(**share):
+        a = {n: own[share.get(n, n)].data_ptr() for n in names}
+        st = lib.kessie_step_tables(a["table"], 8, 8, a["computed"], a["new"], a["delta"], a["free"], a["count"], 5, 2, 16, 4, a["starts"],
+                                    a["lens"], a["slots"], a["pos"], a["taken"], a["valid"], a["where"], 5, None)
+        return st, _lib.last_error()[1]
+    for out in ("table", "starts", "lens", "slots", "pos", "taken", "valid", "where"):
+        for other in names:
+            if other != out:
+                st, msg = status(**{out: other})
+                assert st == _lib.ERR_INVALID and "over" in msg, (out, other)
