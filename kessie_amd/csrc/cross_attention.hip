@@ -241,9 +241,33 @@ struct Core {
   }
   // O^T += V^T P^T over the 32 states whose V lies at `base`.  Returns the sum of this lane's p as the product took
   // them (16-bit types: rounded to T, so that the weights that V meets are the ones that the sum normalises).
+  // kAhead: with fp32's operands read a group ahead, in this order (the compiler's own, with little else to do between,
+  // waits for each: 32 x 1 on 1,500, 16 heads of 64, 97 us against 83).
+  template <bool kAhead>
   __device__ __forceinline__ float add(uint32_t base, const f32x16& p, f32x16 (&o)[DB]) const {
     float sum = 0.0f;
-    if constexpr (kF32) {
+    if constexpr (kF32 && kAhead) {
+      float v[2][4][DB];
+      auto read = [&](int g) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) v[g & 1][i][db] = lds_read<float>(base + va[db] + (uint32_t)((8 * g + i) * RB));
+      };
+      read(0);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if (g < 3) read(g + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sum += p[4 * g + i];
+#pragma unroll
+          for (int db = 0; db < DB; ++db) o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[g & 1][i][db], p[4 * g + i], o[db], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else if constexpr (kF32) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         sum += p[i];
@@ -646,7 +670,7 @@ __global__ __launch_bounds__(NW * 64) void cross_rows_kernel(Args a) {
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[nb][i] = __builtin_amdgcn_exp2f(fmaf(s[nb][i], a.c2, -use));
-      l += core.add(at + kTile + (uint32_t)(32 * nb * C::RB), s[nb], o);
+      l += core.template add<true>(at + kTile + (uint32_t)(32 * nb * C::RB), s[nb], o);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this stage is read
     issue(t + 2, stage);
@@ -803,22 +827,9 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   uint64_t bits = 0, bits1 = 0;  // the states of tiles t and t + 1
   int byte = 0;                  // this lane's mask byte of tile t + 2
   float high = 0.0f;             // this lane's largest score of tile t, before any are hidden
-  auto iteration = [&](int t, f32x16 (&s)[2], f32x16 (&sn)[2], const int par) {  // par = t % 2
-    const uint64_t bits2 = seen(t + 2, byte);
-    byte = mask_byte(t + 3);
-    issue_k(t + 2, par);
-    issue_v(t + 1, par ^ 1, bits1);
-    const uint32_t kn = lds0 + (par ^ 1) * kTile, vn = lds0 + (2 + par) * kTile;
-    if (bits != ~0ull) {
-      C::hide(s[0], (uint32_t)bits, half);
-      C::hide(s[1], (uint32_t)(bits >> 32), half);
-      high = fmaxf(C::top(s[0]), C::top(s[1]));
-    }
-    bits = bits1;
-    bits1 = bits2;
-    const float top = max_halves(high) * c2;
+  // The maximum with this tile's; returns what is taken from the scores.
+  auto rescale = [&](float top) {
     const float mn = top > m + kSlack ? top : m;
-    const float use = mn == kNegInf ? 0.0f : mn;
     const float alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
     if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
 #pragma unroll
@@ -826,16 +837,40 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
       l *= alpha;
     }
     m = mn;
+    return mn == kNegInf ? 0.0f : mn;
+  };
+  auto hide_both = [&](f32x16 (&s)[2], uint64_t seen) {
+    C::hide(s[0], (uint32_t)seen, half);
+    C::hide(s[1], (uint32_t)(seen >> 32), half);
+  };
+  auto largest = [](const f32x16 (&s)[2]) { return fmaxf(C::top(s[0]), C::top(s[1])); };
+  auto iteration = [&](int t, f32x16 (&s)[2], f32x16 (&sn)[2], const int par) {  // par = t % 2
+    const uint64_t bits2 = seen(t + 2, byte);
+    byte = mask_byte(t + 3);
+    issue_k(t + 2, par);
+    issue_v(t + 1, par ^ 1, bits1);
+    const uint32_t kn = lds0 + (par ^ 1) * kTile, vn = lds0 + (2 + par) * kTile;
+    if (bits != ~0ull) {
+      hide_both(s, bits);
+      high = largest(s);
+    }
+    bits = bits1;
+    bits1 = bits2;
+    const float use = rescale(max_halves(high) * c2);
     if constexpr (C::kF32) {
-      sn[0] = core.scores(kn, q);
-      sn[1] = core.scores(kn + 32 * C::RB, q);
+      // (Scores of no tile are left out at head_dim 64; at 128, where one wave a SIMD is all that the registers leave, a
+      // branch here keeps them from running beside the softmax: 2 x 1,000 on 4,000, 8 heads, 387 us against 345.)
+      if (D == 128 || t + 1 < n) {
+        sn[0] = core.scores(kn, q);
+        sn[1] = core.scores(kn + 32 * C::RB, q);
+      }
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[nb][i] = __builtin_amdgcn_exp2f(fmaf(s[nb][i], c2, -use));
-        l += core.add(vn + (uint32_t)(32 * nb * C::RB), s[nb], o);
+        l += core.template add<false>(vn + (uint32_t)(32 * nb * C::RB), s[nb], o);
       }
-      high = fmaxf(C::top(sn[0]), C::top(sn[1]));
+      high = largest(sn);
     } else {
       // Steps: the MFMAs of S^T(t + 1), then those of PV, each with its operand two steps ahead and its share of the
       // 16 score pairs, which go through three stages in three steps -- scaled; exp2; packed and summed -- so that no
@@ -907,7 +942,7 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     f32x16 sa[2], sb[2];
     sa[0] = core.scores(lds0, q);
     sa[1] = core.scores(lds0 + 32 * C::RB, q);
-    high = fmaxf(C::top(sa[0]), C::top(sa[1]));
+    high = largest(sa);
     wait_loads_and_meet();  // (iteration 0 loads over tile 0's K)
     for (int t = 0; t < n; t += 2) {
       iteration(t, sa, sb, 0);
@@ -1142,10 +1177,11 @@ Plan make_plan(int B, int max_q, int Tq, int Hq, int Hkv, int D, int max_kv, int
   Plan p{};
   int keys, per_cu, gain;
   const int nw = row_bytes == 512 ? 2 : 4, rows_per_cu = 160 * 1024 / (nw * 4 * kRowsKeys * row_bytes);
-  // Few rows altogether over few states (at most three tiles a wave): the waves of a workgroup share the states of 32
-  // rows and merge them in LDS.  1 x 40 on 300 (fp32, 8 heads of 64) 15.2 us against 18.5 with 128 rows a workgroup;
-  // past that it loses: 8 x 60 on 1,000 (bf16, 8 heads of 128) 19.9 against 17.1.
-  const bool small = tiles_of(32) * Hkv <= (int64_t)cus * rows_per_cu && max_kv <= 3 * nw * kRowsKeys;
+  // Few rows altogether over few states (at most five tiles a wave, three in fp32): the waves of a workgroup share the
+  // states of 32 rows and merge them in LDS.  1 x 60 on 600 (bf16, 8 heads of 128) 12.3 us against 15.3 with 128 rows a
+  // workgroup, 4 x 50..101 on 300 (fp32, 12 heads of 64) 15.3 against 17.1; past that it loses: 1 x 60 on 1,000 15.7
+  // against 13.6, and in fp32 on 577 21.7 against 20.0.
+  const bool small = tiles_of(32) * Hkv <= (int64_t)cus * rows_per_cu && max_kv <= (es == 4 ? 3 : 5) * nw * kRowsKeys;
   if (most <= 32 || small) {
     p.tiles = most <= 32 ? B : tiles_of(32);
     p.part_rows = (int)(most < 32 ? most : 32);
@@ -1161,8 +1197,11 @@ Plan make_plan(int B, int max_q, int Tq, int Hq, int Hkv, int D, int max_kv, int
     const int rows = p.waves * 32;
     p.tiles = tiles_of(rows);
     p.part_rows = (int)(most < rows ? most : rows);
-    p.min_steps = es == 4 ? 2 : 4;
     keys = 64;
+    // fp32: a step is 3 us of MFMA work, so that each may have a workgroup of its own while there are CUs for them: 2 x 60
+    // on 500 (8 heads of 128) 24.6 us against 34.2 with two steps each; 4 x 50..101 on 577 (12 heads of 64) 20.0 with
+    // two, 22.9 with one.
+    p.min_steps = es == 2 ? 4 : p.tiles * Hkv * div_up(max_kv, keys) <= cus ? 1 : 2;
     per_cu = p.waves == 8 || row_bytes == 512 ? 1 : 2;
     gain = es == 4 ? 4 : 14;
   }

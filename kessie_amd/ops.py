@@ -439,13 +439,14 @@ def rope_remap_paged(pool: torch.Tensor, orig_pos: torch.Tensor, tgt_pos: torch.
 # ---------------------------------------------------------------------------
 # Rotary positions with several axes
 # ---------------------------------------------------------------------------
-def _gpu(first: str, **tensors: Optional[torch.Tensor]) -> int:
-    """The GPU that ``tensors[first]`` is on; all others given must be there too (a kernel is handed plain addresses)."""
-    dev = tensors[first].get_device()
+def _gpu(names: str, *tensors: Optional[torch.Tensor]) -> int:
+    """The GPU that the first tensor is on; all others given must be there too (a kernel is handed plain addresses)."""
+    dev = tensors[0].get_device()
     if dev < 0:
-        raise ValueError(f"{first} must be on the GPU, got {tensors[first].device}")
-    for name, t in tensors.items():
+        raise ValueError(f"{names.split()[0]} must be on the GPU, got {tensors[0].device}")
+    for t in tensors:
         if t is not None and t.get_device() != dev:
+            name = next(n for n, x in zip(names.split(), tensors) if x is t)
             raise ValueError(f"{name} is on {t.device}, not on cuda:{dev}")
     return dev
 
@@ -455,7 +456,7 @@ _here = contextlib.nullcontext()
 
 def _on(dev: int):
     """GPU ``dev`` made current for a launch (nothing to do where it is already)."""
-    return _here if torch.cuda.current_device() == dev else torch.cuda.device(dev)
+    return _here if torch._C._cuda_getDevice() == dev else torch.cuda.device(dev)
 
 
 def _raw_stream(stream, dev: int) -> int:
@@ -548,7 +549,7 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
         raise ValueError("k_out without k")
     row = _positions_arg(positions, len(sections), t, "positions")
     r = _inv_arg(inv_freq, d)
-    dev = _gpu("q", q=q, k=k, q_out=q_out, k_out=k_out, positions=positions, inv_freq=inv_freq)
+    dev = _gpu("q k q_out k_out positions inv_freq", q, k, q_out, k_out, positions, inv_freq)
     (qs0, qs1, _), (qo0, qo1, _) = q.stride(), q_out.stride()
     with _on(dev):
         _lib.check("kessie_rope_axes", _lib.load().kessie_rope_axes(
@@ -588,8 +589,7 @@ def rope_axes_cache_write(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.T
         raise ValueError("slot_mapping must be int64 with one entry per token")
     row = _positions_arg(positions, len(sections), t, "positions")
     r = _inv_arg(inv_freq, d)
-    dev = _gpu("pool", pool=pool, q=q, q_out=q_out, k=k, v=v, positions=positions, slot_mapping=slot_mapping,
-               inv_freq=inv_freq)
+    dev = _gpu("pool q q_out k v positions slot_mapping inv_freq", pool, q, q_out, k, v, positions, slot_mapping, inv_freq)
     _contig(slot_mapping, "slot_mapping")
     (ks0, ks1, _), (vs0, vs1, _) = k.stride(), v.stride()
     with _on(dev):
@@ -625,7 +625,7 @@ def rope_remap_axes(pool: torch.Tensor, orig_pos: torch.Tensor, tgt_pos: torch.T
         if page_list.numel() * p_size < t:
             raise ValueError("page_list too short for the token count")
     r = _inv_arg(inv_freq, d)
-    dev = _gpu("pool", pool=pool, orig_pos=orig_pos, tgt_pos=tgt_pos, inv_freq=inv_freq, page_list=page_list)
+    dev = _gpu("pool orig_pos tgt_pos inv_freq page_list", pool, orig_pos, tgt_pos, inv_freq, page_list)
     with _on(dev):
         _lib.check("kessie_rope_remap_axes", _lib.load().kessie_rope_remap_axes(
             pool.data_ptr(), ps, ts, hs, _addr(page_list), n_pages, orig_pos.data_ptr(), r0, tgt_pos.data_ptr(), r1,
@@ -680,8 +680,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_sta
         out = torch.empty(t, hq, d, dtype=q.dtype, device=q.device)
     else:
         _rows3(out, "out", q.shape, q.dtype)
-    dev = _gpu("q", q=q, k=k, v=v, query_start_loc=query_start_loc, kv_start=kv_start, kv_lens=kv_lens, key_mask=key_mask,
-               out=out, ws=ws)
+    dev = _gpu("q k v query_start_loc kv_start kv_lens key_mask out ws",
+               q, k, v, query_start_loc, kv_start, kv_lens, key_mask, out, ws)
     if not (query_start_loc.is_contiguous() and kv_start.is_contiguous() and kv_lens.is_contiguous()):
         raise ValueError("query_start_loc, kv_start and kv_lens must be contiguous")
     dt = dtype_code(q.dtype)
@@ -776,9 +776,9 @@ def step_tables(block_table: torch.Tensor, computed_lens: torch.Tensor, new_lens
                 and lens.is_contiguous() and slots.is_contiguous() and pos.is_contiguous()):
             raise ValueError(f"out must be contiguous int32 [{b + 1}], int32 [{b}], int64 [{num_token_rows}], int32 "
                              f"[{num_token_rows}], int32 [1], got {[(x.dtype, tuple(x.shape)) for x in out]}")
-    dev = _gpu("block_table", block_table=block_table, computed_lens=computed_lens, new_lens=new_lens, free_pages=free_pages,
-               free_count=free_count, position_delta=position_delta, page_valid=page_valid, page_positions=page_positions,
-               query_start_loc=out[0], seq_lens=out[1], slot_mapping=out[2], positions=out[3], taken=out[4])
+    dev = _gpu("block_table computed_lens new_lens free_pages free_count position_delta page_valid page_positions "
+               "query_start_loc seq_lens slot_mapping positions taken",
+               block_table, computed_lens, new_lens, free_pages, free_count, position_delta, page_valid, page_positions, *out)
     if not (computed_lens.is_contiguous() and new_lens.is_contiguous()):
         raise ValueError("computed_lens and new_lens must be contiguous")
     for name, t in (("free_pages", free_pages), ("position_delta", position_delta), ("page_valid", page_valid),
