@@ -6,7 +6,8 @@
 // over the states j of t's sequence that key_mask leaves; no state, zeros.
 //
 // A row is a (query, head) pair: the C * G rows of one (sequence, kv head) are
-// packed, since they read the same states.  Two kernels share one core, which
+// packed, since they read the same states.  cross_rows_kernel (few rows: HBM or
+// latency bound) and cross_tile_kernel (many: MFMA bound) share one core, which
 // takes 32 rows and 32 states at a time:
 //
 //   S^T = K Q^T   v_mfma_f32_32x32x16 (fp32: 32x32x2), states x rows: lane l
@@ -63,9 +64,9 @@ struct Args {
   // at a scale of zero); a negative scale flips q instead (flip).
   float c2;
   int flip;
-  // Work split over the states: `shares` workgroups per kv head wanted, each of at least
-  // min_steps steps.  plan: what the main kernel's first workgroup leaves for the merge.  Partials
-  // of part_rows rows each: unnormalised sums [rows][D], base-2 maxima and sums.
+  // Work split over the states: `shares` workgroups per kv head wanted, each of at least min_steps steps.  plan: what the
+  // main kernel's first workgroup leaves for the merge (each sequence's first step; the tile kernel, the pieces' length).
+  // Partials of part_rows rows each: unnormalised sums [rows][D], base-2 maxima and sums.
   int shares, min_steps, part_rows;
   int64_t* plan;
   float* ws_o;
@@ -196,7 +197,8 @@ struct Core {
   // Q of this lane's row as the B operand: 16-bit, step s holds d = 16 s + 8 half ..; fp32, step s
   // d = half * D / 2 + s (the order of d within the product is free).
   static constexpr int QN = kF32 ? D / 8 : D / 16;
-  typedef typename std::conditional<kF32, f32x4, typename std::conditional<kF32, bf16x8, typename Half<typename std::conditional<kF32, bf16_t, T>::type>::v8>::type>::type QV;
+  typedef typename Half<typename std::conditional<kF32, bf16_t, T>::type>::v8 Half8;
+  typedef typename std::conditional<kF32, f32x4, Half8>::type QV;
   static __device__ __forceinline__ int q_elem(int s, int half) { return kF32 ? half * (D / 2) + 4 * s : 16 * s + 8 * half; }
 
   uint32_t ka[QN];  // LDS offsets of K's operands of a 32-state block
@@ -204,7 +206,8 @@ struct Core {
   __device__ __forceinline__ void init(int lane) {
     const int col = lane & 31, half = lane >> 5;
 #pragma unroll
-    for (int s = 0; s < QN; ++s) ka[s] = (uint32_t)(col * RB + (((kF32 ? half * (CH / 2) + s : 2 * s + half) ^ k_swizzle(col)) * 16));
+    for (int s = 0; s < QN; ++s)
+      ka[s] = (uint32_t)(col * RB + (((kF32 ? half * (CH / 2) + s : 2 * s + half) ^ k_swizzle(col)) * 16));
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
       if (kF32) {
@@ -334,7 +337,7 @@ __device__ __forceinline__ i32x4 tile_rsrc(const char* base, int rows, int ts_b,
                kRsrcWord3};
 }
 
-// Which states of a tile are there and not hidden, one bit each.  With a mask,
+// Which states of a tile of cross_rows_kernel are there and not hidden, one bit each.  With a mask,
 // lane i keeps the bits of tile 64 n + i of this wave's tiles and loads the next
 // 64 tiles' when they are asked for (in rising order).
 template <bool kMask, int KT>
@@ -590,8 +593,14 @@ __device__ __forceinline__ void store_row(T* row, const f32x16 (&o)[D / 32], flo
 }
 
 // 32 rows of a (sequence, kv head): decoding, and prompts too small to fill the
-// device with larger tiles.  A step is NW tiles, one a wave; every wave streams its tiles through two LDS stages of its own, the next
-// tile in flight while one is computed: no barrier before the merge.  Bound: HBM.
+// device with larger tiles.  A step is NW tiles, one a wave; every wave streams
+// its tiles through two LDS stages of its own, the next tile in flight while one
+// is computed: no barrier before the merge.
+//
+// Decoding is bound by HBM.  16 x 1 query over 6,400 to 25,600 states (64 / 8
+// heads of 128, bf16, 0.92 GB) 151 us with the combine = 6.1 TB/s, 88 % of what
+// this card's best reads reach; 32 x 1 over 1,500 (16 heads of 64, 0.2 GB) 37 us
+// = 5.3 TB/s, 4 of them the combine.
 template <typename T, int D, int KT, int NW, bool kMask, bool kShare>
 __global__ __launch_bounds__(NW * 64) void cross_rows_kernel(Args a) {
   typedef Core<T, D> C;
@@ -609,128 +618,128 @@ __global__ __launch_bounds__(NW * 64) void cross_rows_kernel(Args a) {
   C core;
   core.init(lane);
   do {
-  const Stretch now = uniform(walk.now);
-  const Seq sq = now.sq;
-  const int row0 = now.rt * 32, rows = min(sq.nq * a.G - row0, 32);
-  typename C::QV q[C::QN];
-  C::load_q(a, sq, row0 + min(col, rows - 1), g, half, q, col < rows);
-  const char* kbase = static_cast<const char*>(a.k) + ((int64_t)sq.kv0 * a.k_ts + (int64_t)g * a.k_hs) * (int64_t)sizeof(T);
-  const char* vbase = static_cast<const char*>(a.v) + ((int64_t)sq.kv0 * a.v_ts + (int64_t)g * a.v_hs) * (int64_t)sizeof(T);
-  const int nkv = (int)min((int64_t)sq.nkv, (int64_t)now.end * (NW * KT));  // states up to this stretch's end
-  const int first = now.t * NW + wave, step = NW;
-  const int n = uniform(max(div_up(div_up(nkv, KT) - first, step), 0));
-  Seen<kMask, KT> seen{kMask ? a.mask + sq.kv0 : nullptr, nkv, first, step, 0};
-  const uint32_t mine = lds0 + (uint32_t)wave * 4 * kTile;  // this wave's stages: K, V, K, V
+    const Stretch now = uniform(walk.now);
+    const Seq sq = now.sq;
+    const int row0 = now.rt * 32, rows = min(sq.nq * a.G - row0, 32);
+    typename C::QV q[C::QN];
+    C::load_q(a, sq, row0 + min(col, rows - 1), g, half, q, col < rows);
+    const char* kbase = static_cast<const char*>(a.k) + ((int64_t)sq.kv0 * a.k_ts + (int64_t)g * a.k_hs) * (int64_t)sizeof(T);
+    const char* vbase = static_cast<const char*>(a.v) + ((int64_t)sq.kv0 * a.v_ts + (int64_t)g * a.v_hs) * (int64_t)sizeof(T);
+    const int nkv = (int)min((int64_t)sq.nkv, (int64_t)now.end * (NW * KT));  // states up to this stretch's end
+    const int first = now.t * NW + wave, step = NW;
+    const int n = uniform(max(div_up(div_up(nkv, KT) - first, step), 0));
+    Seen<kMask, KT> seen{kMask ? a.mask + sq.kv0 : nullptr, nkv, first, step, 0};
+    const uint32_t mine = lds0 + (uint32_t)wave * 4 * kTile;  // this wave's stages: K, V, K, V
 
-  uint64_t bits[2];
-  auto issue = [&](int t, int stage) {
-    const uint64_t at = seen.at(t, lane);
-    bits[stage] = at;
-    const int tile = first + t * step, r = seen.rows(t);
-    const i32x4 kr = tile_rsrc(kbase + (int64_t)tile * KT * ts_k, r, ts_k, C::RB);
-    const i32x4 vr = tile_rsrc(vbase + (int64_t)tile * KT * ts_v, r, ts_v, C::RB);
-    const uint32_t to = mine + (uint32_t)stage * 2 * kTile;
+    uint64_t bits[2];
+    auto issue = [&](int t, int stage) {
+      const uint64_t at = seen.at(t, lane);
+      bits[stage] = at;
+      const int tile = first + t * step, r = seen.rows(t);
+      const i32x4 kr = tile_rsrc(kbase + (int64_t)tile * KT * ts_k, r, ts_k, C::RB);
+      const i32x4 vr = tile_rsrc(vbase + (int64_t)tile * KT * ts_v, r, ts_v, C::RB);
+      const uint32_t to = mine + (uint32_t)stage * 2 * kTile;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) stream_to_lds(kr, C::k_offset(i, lane, ts_k), uniform(to + 1024u * i));
+      for (int i = 0; i < NI; ++i) stream_to_lds(kr, C::k_offset(i, lane, ts_k), uniform(to + 1024u * i));
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      uint32_t off = C::v_offset(i, lane, ts_v);
-      // (A hidden state's V arrives as zeros, whatever it holds.)
-      if (kMask && !((at >> (i * C::RPI + lane / C::CH)) & 1)) off = 0xffffff00u;
-      stream_to_lds(vr, off, uniform(to + kTile + 1024u * i));
-    }
-  };
-
-  f32x16 o[C::DB];
-#pragma unroll
-  for (int i = 0; i < C::DB; ++i) o[i] = f32x16{};
-  float m = kNegInf, l = 0.0f;
-  auto tile = [&](int t, int stage) {
-    wait_loads<2 * NI>();
-    const uint32_t at = mine + (uint32_t)stage * 2 * kTile;
-    f32x16 s[NB];
-    float top = kNegInf;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      s[nb] = core.scores(at + (uint32_t)(32 * nb * C::RB), q);
-      const uint32_t some = (uint32_t)(bits[stage] >> (32 * nb));
-      if (some != 0xffffffffu) C::hide(s[nb], some, half);
-      top = fmaxf(top, C::top(s[nb]));
-    }
-    const float mn = fmaxf(m, max_halves(top) * a.c2);
-    const float use = mn == kNegInf ? 0.0f : mn;
-    const float alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-    m = mn;
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
-#pragma unroll
-      for (int i = 0; i < C::DB; ++i) o[i] *= alpha;
-      l *= alpha;
-    }
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[nb][i] = __builtin_amdgcn_exp2f(fmaf(s[nb][i], a.c2, -use));
-      l += core.template add<true>(at + kTile + (uint32_t)(32 * nb * C::RB), s[nb], o);
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this stage is read
-    issue(t + 2, stage);
-  };
-  if (n > 0) {
-    issue(0, 0);
-    issue(1, 1);
-    C::flip_q(a, q);
-    for (int t = 0; t < n; t += 2) {
-      tile(t, 0);
-      if (t + 1 < n) tile(t + 1, 1);
-    }
-  }
-  l = sum_halves(l);
-
-  // The waves' (o, m, l) meet in LDS, in wave order.
-  wait_loads_and_meet();
-  float* so = reinterpret_cast<float*>(smem);
-  float* sm = so + NW * 32 * kOut;
-  float* sl = sm + NW * 32;
-  if (col < rows) {
-    store_row<float, D>(so + (wave * 32 + col) * kOut, o, 1.0f, half);
-    if (half == 0) {
-      sm[wave * 32 + col] = m;
-      sl[wave * 32 + col] = l;
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * (D / 4); i += NW * 64) {
-    const int r = i / (D / 4), d = 4 * (i % (D / 4));
-    float top = sm[r];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) top = fmaxf(top, sm[w * 32 + r]);
-    const float use = top == kNegInf ? 0.0f : top;
-    f32x4 y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float e = __builtin_amdgcn_exp2f(sm[w * 32 + r] - use);
-      sum += e * sl[w * 32 + r];
-      if (e != 0.0f) y += e * *reinterpret_cast<const f32x4*>(so + (w * 32 + r) * kOut + d);
-    }
-    const int pos = (unsigned)(row0 + r) / (unsigned)a.G, h = g * a.G + row0 + r - pos * a.G;
-    if (kShare && !(now.t == 0 && now.end == now.steps)) {
-      const int64_t row = part_row(a, now.t == 0, r);
-      *reinterpret_cast<f32x4*>(a.ws_o + row * D + d) = y;
-      if (d == 0) {
-        a.ws_m[row] = top;
-        a.ws_l[row] = sum;
+      for (int i = 0; i < NI; ++i) {
+        uint32_t off = C::v_offset(i, lane, ts_v);
+        // (A hidden state's V arrives as zeros, whatever it holds.)
+        if (kMask && !((at >> (i * C::RPI + lane / C::CH)) & 1)) off = 0xffffff00u;
+        stream_to_lds(vr, off, uniform(to + kTile + 1024u * i));
       }
-    } else {
-      typedef T V __attribute__((ext_vector_type(4)));
-      const float il = sum != 0.0f ? 1.0f / sum : 0.0f;
-      V z;
+    };
+
+    f32x16 o[C::DB];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[e] = from_f32<T>(y[e] * il);
-      *reinterpret_cast<V*>(static_cast<T*>(a.out) + (int64_t)(sq.q0 + pos) * a.o_ts + (int64_t)h * a.o_hs + d) = z;
+    for (int i = 0; i < C::DB; ++i) o[i] = f32x16{};
+    float m = kNegInf, l = 0.0f;
+    auto tile = [&](int t, int stage) {
+      wait_loads<2 * NI>();
+      const uint32_t at = mine + (uint32_t)stage * 2 * kTile;
+      f32x16 s[NB];
+      float top = kNegInf;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        s[nb] = core.scores(at + (uint32_t)(32 * nb * C::RB), q);
+        const uint32_t some = (uint32_t)(bits[stage] >> (32 * nb));
+        if (some != 0xffffffffu) C::hide(s[nb], some, half);
+        top = fmaxf(top, C::top(s[nb]));
+      }
+      const float mn = fmaxf(m, max_halves(top) * a.c2);
+      const float use = mn == kNegInf ? 0.0f : mn;
+      const float alpha = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+#pragma unroll
+        for (int i = 0; i < C::DB; ++i) o[i] *= alpha;
+        l *= alpha;
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[nb][i] = __builtin_amdgcn_exp2f(fmaf(s[nb][i], a.c2, -use));
+        l += core.template add<true>(at + kTile + (uint32_t)(32 * nb * C::RB), s[nb], o);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this stage is read
+      issue(t + 2, stage);
+    };
+    if (n > 0) {
+      issue(0, 0);
+      issue(1, 1);
+      C::flip_q(a, q);
+      for (int t = 0; t < n; t += 2) {
+        tile(t, 0);
+        if (t + 1 < n) tile(t + 1, 1);
+      }
     }
-  }
-  if (kShare) __syncthreads();  // (the next stretch loads over the merge)
+    l = sum_halves(l);
+
+    // The waves' (o, m, l) meet in LDS, in wave order.
+    wait_loads_and_meet();
+    float* so = reinterpret_cast<float*>(smem);
+    float* sm = so + NW * 32 * kOut;
+    float* sl = sm + NW * 32;
+    if (col < rows) {
+      store_row<float, D>(so + (wave * 32 + col) * kOut, o, 1.0f, half);
+      if (half == 0) {
+        sm[wave * 32 + col] = m;
+        sl[wave * 32 + col] = l;
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * (D / 4); i += NW * 64) {
+      const int r = i / (D / 4), d = 4 * (i % (D / 4));
+      float top = sm[r];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) top = fmaxf(top, sm[w * 32 + r]);
+      const float use = top == kNegInf ? 0.0f : top;
+      f32x4 y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float e = __builtin_amdgcn_exp2f(sm[w * 32 + r] - use);
+        sum += e * sl[w * 32 + r];
+        if (e != 0.0f) y += e * *reinterpret_cast<const f32x4*>(so + (w * 32 + r) * kOut + d);
+      }
+      const int pos = (unsigned)(row0 + r) / (unsigned)a.G, h = g * a.G + row0 + r - pos * a.G;
+      if (kShare && !(now.t == 0 && now.end == now.steps)) {
+        const int64_t row = part_row(a, now.t == 0, r);
+        *reinterpret_cast<f32x4*>(a.ws_o + row * D + d) = y;
+        if (d == 0) {
+          a.ws_m[row] = top;
+          a.ws_l[row] = sum;
+        }
+      } else {
+        typedef T V __attribute__((ext_vector_type(4)));
+        const float il = sum != 0.0f ? 1.0f / sum : 0.0f;
+        V z;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = from_f32<T>(y[e] * il);
+        *reinterpret_cast<V*>(static_cast<T*>(a.out) + (int64_t)(sq.q0 + pos) * a.o_ts + (int64_t)h * a.o_hs + d) = z;
+      }
+    }
+    if (kShare) __syncthreads();  // (the next stretch loads over the merge)
   } while (walk.next(a, 32, NW * KT));
 }
 
@@ -754,6 +763,14 @@ constexpr float kSlack = 8.0f;
 // softmax of tile t in the shadow of S^T(t + 1), then O^T += V^T P^T(t); one
 // barrier.  Each MFMA is issued with its share of the other work and its
 // operands two steps ahead, in a fixed order (a scheduling barrier a step).
+//
+// 4,096 queries over 16,384 states (32 / 8 heads of 128, bf16, 1.1 TFLOP): 953 us
+// = 1,154 TFLOP/s, 85 % of a large library product; the MFMA pipes are 63 % busy
+// at the 1.64 GHz that power leaves, LDS 32 %, no bank conflicts.  More stages or
+// operands read 3 to 8 steps ahead changed nothing: a wave's issue bounds a step
+// (its MFMA, operand reads and a share of the softmax, 52 to 65 cycles, beside
+// the other wave's).  2 x 2,048 over 4,096 (16 heads of 64): 79 us, 870 TFLOP/s,
+// where the 32 exp2 of a lane take as long as the MFMAs.
 template <typename T, int D, int W, bool kMask, bool kShare>
 __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void cross_tile_kernel(Args a) {
   typedef Core<T, D> C;
@@ -876,7 +893,8 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
       // 16 score pairs, which go through three stages in three steps -- scaled; exp2; packed and summed -- so that no
       // stage waits for the one before; a pair is packed before the PV step that takes it.  The last steps take the
       // next tile's largest score.
-      constexpr int kQ = 2 * C::QN, kPV = 4 * C::DB, kSpread = kQ + 3 * C::DB - 2, kMaxAt = kQ + 4, kMaxPer = 16 / (kPV - 4) + (16 % (kPV - 4) != 0);
+      constexpr int kQ = 2 * C::QN, kPV = 4 * C::DB, kSpread = kQ + 3 * C::DB - 2;
+      constexpr int kMaxAt = kQ + 4, kMaxPer = 16 / (kPV - 4) + (16 % (kPV - 4) != 0);
       static_assert(kQ + 3 * C::DB >= kSpread + 2, "the last pairs are packed in time");
       u32x4 w[4];  // p as V^T's partner: w[c] of states 16 c ..
       float l0 = 0.0f, l1 = 0.0f;
@@ -930,7 +948,21 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     }
     wait_loads_and_meet();
   };
-  if (n > 0) {
+  if (n > 0 && now.rt * kRows + wave * 32 >= rows) {
+    // A wave without rows only loads its part of the tiles (13 x 21..701 on 640..6,404, 97 us -> 95).
+    bits1 = seen(0, mask_byte(0));
+    issue_k(0, 0);
+    issue_v(0, 0, bits1);
+    issue_k(1, 1);
+    wait_loads_and_meet();
+    wait_loads_and_meet();
+    for (int t = 0; t < n; ++t) {
+      bits1 = seen(t + 1, mask_byte(t + 1));
+      issue_k(t + 2, t & 1);
+      issue_v(t + 1, (t + 1) & 1, bits1);
+      wait_loads_and_meet();
+    }
+  } else if (n > 0) {
     bits = seen(0, mask_byte(0));
     bits1 = seen(1, mask_byte(1));
     byte = mask_byte(2);
@@ -953,7 +985,8 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   if (row < rows) {
     const int pos = (unsigned)row / (unsigned)a.G, h = g * a.G + row - pos * a.G;
     if (!kShare || now.pieces == 1) {
-      store_row<T, D>(static_cast<T*>(a.out) + (int64_t)(sq.q0 + pos) * a.o_ts + (int64_t)h * a.o_hs, o, l != 0.0f ? 1.0f / l : 0.0f, half);
+      T* to = static_cast<T*>(a.out) + (int64_t)(sq.q0 + pos) * a.o_ts + (int64_t)h * a.o_hs;
+      store_row<T, D>(to, o, l != 0.0f ? 1.0f / l : 0.0f, half);
     } else {
       const int64_t r = (int64_t)blockIdx.x * a.part_rows + wave * 32 + col;
       store_row<float, D>(a.ws_o + r * D, o, 1.0f, half);
@@ -1068,7 +1101,9 @@ __global__ __launch_bounds__(256) void cross_combine_kernel(Args a, int rows_per
     }
     if (j0 == j1 || h0 + sub >= h_end) continue;  // stored already
     // Partial of workgroup j: number 1 of the first, 0 of those after it.
-    const f32x4 y = merge_partials<D>(a, j1 - j0 + 1, d, [&](int i) { return (((int64_t)(j0 + i) * a.Hkv + g) * 2 + (i == 0)) * a.part_rows + r; });
+    const f32x4 y = merge_partials<D>(a, j1 - j0 + 1, d, [&](int i) {
+      return (((int64_t)(j0 + i) * a.Hkv + g) * 2 + (i == 0)) * a.part_rows + r;
+    });
     store4(static_cast<T*>(a.out) + (int64_t)t * a.o_ts + (int64_t)h * a.o_hs + d, y);
   }
 }
@@ -1209,7 +1244,8 @@ Plan make_plan(int B, int max_q, int Tq, int Hq, int Hkv, int D, int max_kv, int
   // Split where the longest sequence would outlast an even share of the work by more than the merge costs (`gain`
   // steps: 5 us of it in decoding, 10 otherwise).  What an even share is goes by the means that the host knows.
   const int64_t slots = (int64_t)cus * per_cu;
-  const double mean = B > 0 && Tkv / B < max_kv ? (double)Tkv / B : max_kv, tiles = p.waves ? (double)Tq * G / (p.waves * 32) + 0.5 * B : B;
+  const double mean = B > 0 && Tkv / B < max_kv ? (double)Tkv / B : max_kv;
+  const double tiles = p.waves ? (double)Tq * G / (p.waves * 32) + 0.5 * B : B;
   const double even = (tiles < p.tiles ? tiles : (double)p.tiles) * Hkv * (mean / keys + 0.5) / (double)slots;
   if (div_up(max_kv, keys) - even >= gain) {
     p.shares = (int)((slots + Hkv - 1) / Hkv);
@@ -1303,7 +1339,8 @@ extern "C" size_t kessie_cross_attention_workspace_bytes(int batch, int max_quer
   if (batch <= 0 || max_query_len <= 0 || num_q_tokens <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || max_kv_len < 0 ||
       num_kv_tokens < 0 || (head_dim != 64 && head_dim != 128) || dtype_size(dtype) <= 0)
     return 0;
-  const Plan p = make_plan(batch, max_query_len, num_q_tokens, num_q_heads, num_kv_heads, head_dim, max_kv_len, num_kv_tokens, dtype_size(dtype));
+  const Plan p = make_plan(batch, max_query_len, num_q_tokens, num_q_heads, num_kv_heads, head_dim, max_kv_len, num_kv_tokens,
+                           dtype_size(dtype));
   return layout(p, batch, num_kv_heads, head_dim).bytes;
 }
 
