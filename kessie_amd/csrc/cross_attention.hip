@@ -757,6 +757,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // maximum rises by more.
 constexpr float kSlack = 8.0f;
 
+// States of a tile of cross_tile_kernel: 64 KiB of LDS or 32, so that two workgroups of four waves share a CU, and each
+// SIMD has one's softmax to run beside the other's MFMAs (fp32, head_dim 128: 2 x 1,000 on 4,000, 8 heads, 267 us against 344 with one).
+__host__ __device__ constexpr int tile_keys(int row_bytes) { return row_bytes == 512 ? 32 : 64; }
+
 // Prompts: W waves of 32 rows each over tiles of 64 states that the workgroup
 // loads together, two stages of K and of V.  Iteration t asks for K of tile t + 2
 // and V of tile t + 1 (their stages were read in iteration t - 1), runs the
@@ -775,7 +779,7 @@ template <typename T, int D, int W, bool kMask, bool kShare>
 __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void cross_tile_kernel(Args a) {
   typedef Core<T, D> C;
   typedef typename C::QV QV;
-  constexpr int KT = 64;
+  constexpr int KT = tile_keys(C::RB), NB = KT / 32;
   constexpr int NI = KT / C::RPI / W;  // load instructions of a wave for a K (or V) tile
   constexpr uint32_t kTile = KT * C::RB;
   constexpr int kRows = W * 32;
@@ -813,7 +817,7 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   };
   auto seen = [&](int t, int byte) {
     const int n = rows_of(t);
-    const uint64_t there = n >= 64 ? ~0ull : (1ull << n) - 1ull;
+    const uint64_t there = n >= 64 ? ~0ull : (1ull << n) - 1ull;  // (KT == 32: n is 32 at most)
     return kMask ? there & __builtin_amdgcn_ballot_w64(byte != 0) : there;
   };
   // Stages: K, K, V, V.  Tiles are loaded in order: the next one's place is carried along.
@@ -856,33 +860,33 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     m = mn;
     return mn == kNegInf ? 0.0f : mn;
   };
-  auto hide_both = [&](f32x16 (&s)[2], uint64_t seen) {
-    C::hide(s[0], (uint32_t)seen, half);
-    C::hide(s[1], (uint32_t)(seen >> 32), half);
+  constexpr uint64_t kFull = KT == 64 ? ~0ull : 0xffffffffull;
+  auto hide = [&](f32x16 (&s)[NB], uint64_t seen) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) C::hide(s[nb], (uint32_t)(seen >> (32 * nb)), half);
   };
-  auto largest = [](const f32x16 (&s)[2]) { return fmaxf(C::top(s[0]), C::top(s[1])); };
-  auto iteration = [&](int t, f32x16 (&s)[2], f32x16 (&sn)[2], const int par) {  // par = t % 2
+  auto largest = [](const f32x16 (&s)[NB]) { return NB == 1 ? C::top(s[0]) : fmaxf(C::top(s[0]), C::top(s[NB - 1])); };
+  auto scores = [&](uint32_t base, f32x16 (&s)[NB]) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) s[nb] = core.scores(base + (uint32_t)(32 * nb * C::RB), q);
+  };
+  auto iteration = [&](int t, f32x16 (&s)[NB], f32x16 (&sn)[NB], const int par) {  // par = t % 2
     const uint64_t bits2 = seen(t + 2, byte);
     byte = mask_byte(t + 3);
     issue_k(t + 2, par);
     issue_v(t + 1, par ^ 1, bits1);
     const uint32_t kn = lds0 + (par ^ 1) * kTile, vn = lds0 + (2 + par) * kTile;
-    if (bits != ~0ull) {
-      hide_both(s, bits);
+    if (bits != kFull) {
+      hide(s, bits);
       high = largest(s);
     }
     bits = bits1;
     bits1 = bits2;
     const float use = rescale(max_halves(high) * c2);
     if constexpr (C::kF32) {
-      // (Scores of no tile are left out at head_dim 64; at 128, where one wave a SIMD is all that the registers leave, a
-      // branch here keeps them from running beside the softmax: 2 x 1,000 on 4,000, 8 heads, 387 us against 345.)
-      if (D == 128 || t + 1 < n) {
-        sn[0] = core.scores(kn, q);
-        sn[1] = core.scores(kn + 32 * C::RB, q);
-      }
+      if (t + 1 < n) scores(kn, sn);
 #pragma unroll
-      for (int nb = 0; nb < 2; ++nb) {
+      for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[nb][i] = __builtin_amdgcn_exp2f(fmaf(s[nb][i], c2, -use));
         l += core.template add<false>(vn + (uint32_t)(32 * nb * C::RB), s[nb], o);
@@ -971,9 +975,8 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     issue_k(1, 1);
     C::flip_q(a, q);
     wait_loads_and_meet();
-    f32x16 sa[2], sb[2];
-    sa[0] = core.scores(lds0, q);
-    sa[1] = core.scores(lds0 + 32 * C::RB, q);
+    f32x16 sa[NB], sb[NB];
+    scores(lds0, sa);
     high = largest(sa);
     wait_loads_and_meet();  // (iteration 0 loads over tile 0's K)
     for (int t = 0; t < n; t += 2) {
@@ -1212,11 +1215,11 @@ Plan make_plan(int B, int max_q, int Tq, int Hq, int Hkv, int D, int max_kv, int
   Plan p{};
   int keys, per_cu, gain;
   const int nw = row_bytes == 512 ? 2 : 4, rows_per_cu = 160 * 1024 / (nw * 4 * kRowsKeys * row_bytes);
-  // Few rows altogether over few states (at most five tiles a wave, three in fp32): the waves of a workgroup share the
+  // Few rows altogether over few states (at most five tiles a wave; fp32: two or three): the waves of a workgroup share the
   // states of 32 rows and merge them in LDS.  1 x 60 on 600 (bf16, 8 heads of 128) 12.3 us against 15.3 with 128 rows a
-  // workgroup, 4 x 50..101 on 300 (fp32, 12 heads of 64) 15.3 against 17.1; past that it loses: 1 x 60 on 1,000 15.7
-  // against 13.6, and in fp32 on 577 21.7 against 20.0.
-  const bool small = tiles_of(32) * Hkv <= (int64_t)cus * rows_per_cu && max_kv <= (es == 4 ? 3 : 5) * nw * kRowsKeys;
+  // workgroup, 1 x 300 on 100 (fp32, 8 heads of 128) 16.9 against 22.9; past that it loses: 1 x 60 on 1,000 15.7 against
+  // 13.6, 2 x 60 on 180 in fp32 21.5 against 13.9, 4 x 50..101 on 577 (fp32, 12 heads of 64) 21.7 against 20.0.
+  const bool small = tiles_of(32) * Hkv <= (int64_t)cus * rows_per_cu && max_kv <= (es == 2 ? 5 : row_bytes == 512 ? 2 : 3) * nw * kRowsKeys;
   if (most <= 32 || small) {
     p.tiles = most <= 32 ? B : tiles_of(32);
     p.part_rows = (int)(most < 32 ? most : 32);
@@ -1232,12 +1235,12 @@ Plan make_plan(int B, int max_q, int Tq, int Hq, int Hkv, int D, int max_kv, int
     const int rows = p.waves * 32;
     p.tiles = tiles_of(rows);
     p.part_rows = (int)(most < rows ? most : rows);
-    keys = 64;
-    // fp32: a step is 3 us of MFMA work, so that each may have a workgroup of its own while there are CUs for them: 2 x 60
-    // on 500 (8 heads of 128) 24.6 us against 34.2 with two steps each; 4 x 50..101 on 577 (12 heads of 64) 20.0 with
-    // two, 22.9 with one.
+    keys = tile_keys(row_bytes);
+    // fp32: a step is 3 us of MFMA work, so each may have a workgroup of its own while there are CUs for them: 1 x 60 on
+    // 1,000 (8 heads of 64) 14.2 us against 17.2 with two steps each; past that it loses: 2 x 60 on 900 (8 heads of 128)
+    // 24.2 against 20.9, 4 x 50..101 on 577 (12 heads of 64) 22.5 against 20.0.
     p.min_steps = es == 2 ? 4 : p.tiles * Hkv * div_up(max_kv, keys) <= cus ? 1 : 2;
-    per_cu = p.waves == 8 || row_bytes == 512 ? 1 : 2;
+    per_cu = p.waves == 8 ? 1 : 2;
     gain = es == 4 ? 4 : 14;
   }
   p.grid = p.tiles;
@@ -1271,7 +1274,7 @@ template <typename T, int D, bool kMask, bool kShare>
 int launch_fast(const Args& a, const Plan& p, hipStream_t s) {
   typedef Core<T, D> C;
   const dim3 grid((unsigned)(p.grid * a.Hkv));
-  constexpr size_t tile = (size_t)4 * 64 * C::RB;
+  constexpr size_t tile = (size_t)4 * tile_keys(C::RB) * C::RB;
   if constexpr (!C::kF32) {
     if (p.waves == 8) return launch_lds(cross_tile_kernel<T, D, 8, kMask, kShare>, a, grid, 512, tile, s);
   }
@@ -1290,7 +1293,7 @@ int launch_shared(const Args& a, const Plan& p, hipStream_t s) {
     // 32 rows a workgroup, fewer where that leaves the device idle (each finds its row tile first).
     const int rows_wg = p.tiles * a.Hkv * div_up(p.part_rows, 32) < 2 * attn::device_cus() ? 1024 / D : 32;
     hipLaunchKernelGGL((cross_merge_kernel<T, D>), dim3((unsigned)(p.tiles * a.Hkv), div_up(p.part_rows, rows_wg)), dim3(256), 0, s, a,
-                       p.waves * 32, 64, rows_wg);
+                       p.waves * 32, tile_keys(D * (int)sizeof(T)), rows_wg);
     return check_launch("cross attention (merge)");
   }
   int heads = 256 / D;  // (a wave's at once)
