@@ -208,3 +208,30 @@ def test_a_captured_decode_step(dev):
             assert torch.equal(eager[name], graph[name]), (i, name)
         for x, y in zip(eager["tables"], graph["tables"]):
             assert torch.equal(x, y)
+
+
+def test_both_ways_into_the_cache(dev, monkeypatch):
+    """rope_axes and the backend's own write with the fog on, or rope_axes_cache_write and fog_decode with the same bias:
+    the same cache and the same rows."""
+    from kessie_amd import kessie_attention as ka
+    from kessie_amd import ops
+    state = ka.KeSSieAttentionState()
+    state.update(prompt_len=100, recall_positions={5, 30})
+    monkeypatch.setattr(ka, "KESSIE_STATE", state)
+    monkeypatch.setattr(ka, "_FOG_CACHE", ka._FogCache())
+    inv, lens = inv_freq(D // 2, 10000.0, dev), [60, 17, 128]
+    table = torch.arange(36, dtype=torch.int32, device=dev).view(3, WIDTH)
+    free = torch.arange(36, 40, dtype=torch.int32, device=dev)
+    qkv = randn((3, HQ + 2 * HKV, D), torch.bfloat16, dev, 5)
+    pools = [randn((2, PAGES, P, HKV, D), torch.bfloat16, dev, 1) for _ in range(2)]
+    meta = ka.KeSSieAttentionMetadata.build(table, lens, [1, 1, 1], P, free)
+    assert meta.pages_taken == 1
+    pos = three(meta.positions)
+    q, k, v = qkv[:, :HQ].clone(), qkv[:, HQ:HQ + HKV].clone(), qkv[:, HQ + HKV:]
+    ops.rope_axes(q, k, pos, inv, SECTIONS)
+    one = ka.KeSSieAttentionImpl(HQ, D, D ** -0.5, HKV).forward(None, q.view(3, -1), k, v, pools[0], meta)
+    q2, k2 = qkv[:, :HQ].clone(), qkv[:, HQ:HQ + HKV]
+    ops.rope_axes_cache_write(q2, k2, v, pos, pools[1], meta.slot_mapping, inv, SECTIONS, layout="kv_first")
+    bias = ka._FOG_CACHE.get_fog_bias_rows(meta.seq_lens, meta.max_seq_len, q.device, q.dtype, state.get())
+    two = ops.fog_decode(q2, pools[1], meta.block_table, meta.seq_lens, meta.max_seq_len, fog_bias=bias, layout="kv_first")
+    assert torch.equal(q, q2) and torch.equal(pools[0], pools[1]) and torch.equal(one.view(3, HQ, D), two)
