@@ -398,7 +398,7 @@ size_t kessie_cross_attention_workspace_bytes(int batch, int max_query_len,
  * [0, num_kv_tokens) is cut there).  key_mask (NULL: none): one byte a row of
  * k / v, zero hides that state; what k and v hold there is not used, be it NaN.  A
  * query that sees no state gives a zero row.  Rows of out past the last
- * sequence are left as they are.  Element (t, h, d) of q at t*q_tok_stride +
+ * sequence are left as they are; out may be q.  Element (t, h, d) of q at t*q_tok_stride +
  * h*q_head_stride + d, likewise k, v and out (whose rows may not overlap).
  * head_dim <= 256; sums in fp32.  The workspace is written by every call: calls
  * that may overlap need one each. */

@@ -1369,7 +1369,7 @@ extern "C" int kessie_cross_attention(const void* q, int64_t q_tok_stride, int64
   KESSIE_REQUIRE(head_dim <= kMaxD, KESSIE_ERR_UNSUPPORTED, "cross attention: head_dim %d above %d", head_dim, kMaxD);
   KESSIE_REQUIRE(num_q_heads <= 65535, KESSIE_ERR_UNSUPPORTED, "cross attention: %d heads", num_q_heads);
   KESSIE_REQUIRE(dtype_size(dtype) > 0, KESSIE_ERR_UNSUPPORTED, "cross attention: dtype %d", dtype);
-  KESSIE_REQUIRE(fabsf(sm_scale) <= 3.402823466e38f, KESSIE_ERR_INVALID, "cross attention: sm_scale is not finite");
+  KESSIE_REQUIRE(fabsf(sm_scale) * kLog2e <= 3.402823466e38f, KESSIE_ERR_INVALID, "cross attention: sm_scale %g", (double)sm_scale);
   KESSIE_REQUIRE(max_kv_len <= 1 << 30, KESSIE_ERR_UNSUPPORTED, "cross attention: %d states", max_kv_len);
   if (batch == 0 || max_query_len == 0 || num_q_tokens == 0) return KESSIE_OK;
   KESSIE_REQUIRE(q && out && query_start_loc && kv_start && kv_lens && (num_kv_tokens == 0 || (k && v)), KESSIE_ERR_INVALID,

@@ -652,8 +652,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_sta
     ``max_query_len`` and ``max_kv_len`` are host-side upper bounds (longer
     sequences are cut there); key_mask (bool or uint8 [N]) hides states where
     it is zero.  A query without states gives zeros; rows of out behind the
-    last sequence are left as they were.  ws: workspace for split partials (a
-    cached one when None)."""
+    last sequence are left as they were (undefined in a new one).  out may be
+    q.  ws: workspace for split partials (a cached one when None)."""
     _rows3(q, "q")
     t, hq, d = q.shape
     _rows3(k, "k", (k.shape[0], k.shape[1], d), q.dtype)

@@ -344,6 +344,16 @@ def test_kernels_class(dev):
     check(c, got)
 
 
+@pytest.mark.parametrize("seqs,d", [([(1, 60), (1, 9000)], 64), ([(40, 60)] * 2, 128), ([(200, 4000), (3, 5)], 64), ([(700, 900)], 128),
+                                    ([(30, 70)], 80)])
+def test_in_place(dev, seqs, d):
+    """out may be q."""
+    c = case(dev, seqs, 8, 2, d, torch.bfloat16, seed=16, extra_q=0)
+    want = attend(c)
+    q = c["q"].clone()
+    assert attend({**c, "q": q}, out=q) is q and torch.equal(q, want)
+
+
 def test_testing_switches(dev, monkeypatch):
     """KESSIE_FORCE_GENERIC takes the generic kernel, KESSIE_REQUIRE_MFMA refuses what would."""
     from kessie_amd import _lib

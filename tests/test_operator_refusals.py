@@ -149,6 +149,14 @@ def test_rows_of_an_output_that_overlap_are_refused():
     assert rope(64, 0, hq=1) != _lib.OK and "overlap" not in _lib.last_error()[1]
 
 
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), -3e38])
+def test_scales_past_fp32(scale):
+    from kessie_amd import _lib
+    st = _lib.load().kessie_cross_attention(None, 0, 0, None, 0, 0, None, 0, 0, None, None, None, None, None, 0, 0, 1, 1, 1, 1, 1, 4, 2, 64,
+                                            scale, 1, None, 0, None)
+    assert st == _lib.ERR_INVALID and "sm_scale" in _lib.last_error()[1]
+
+
 def test_workspace_of_an_unknown_type():
     from kessie_amd import _lib
     assert _lib.load().kessie_cross_attention_workspace_bytes(1, 1, 1, 60000, 8, 1, 64, 60000, 7) == 0
