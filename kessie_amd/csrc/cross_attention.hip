@@ -770,12 +770,13 @@ __host__ __device__ constexpr int tile_keys(int row_bytes) { return row_bytes ==
 // barrier.  Each MFMA is issued with its share of the other work and its
 // operands two steps ahead, in a fixed order (a scheduling barrier a step).
 //
-// 4,096 queries over 16,384 states (32 / 8 heads of 128, bf16, 1.1 TFLOP): 953 us
-// = 1,154 TFLOP/s, 85 % of a large library product; the MFMA pipes are 63 % busy
+// 4,096 queries over 16,384 states (32 / 8 heads of 128, bf16, 1.1 TFLOP): 916 us
+// = 1,200 TFLOP/s, 89 % of a large library product; the MFMA pipes are 63 % busy
 // at the 1.64 GHz that power leaves, LDS 32 %, no bank conflicts.  More stages or
 // operands read 3 to 8 steps ahead changed nothing: a wave's issue bounds a step
 // (its MFMA, operand reads and a share of the softmax, 52 to 65 cycles, beside
-// the other wave's).  2 x 2,048 over 4,096 (16 heads of 64): 79 us, 870 TFLOP/s,
+// the other wave's), and 64 rows a wave, with nothing beside it, came to 937
+// TFLOP/s.  2 x 2,048 over 4,096 (16 heads of 64): 77 us, 890 TFLOP/s,
 // where the 32 exp2 of a lane take as long as the MFMAs.
 template <typename T, int D, int W, bool kMask, bool kShare>
 __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void cross_tile_kernel(Args a) {
@@ -896,9 +897,10 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
       high = largest(sn);
     } else {
       // Steps: the MFMAs of S^T(t + 1), then those of PV, each with its operand two steps ahead and its share of the
-      // 16 score pairs, which go through three stages in three steps -- scaled; exp2; packed and summed -- so that no
-      // stage waits for the one before; a pair is packed before the PV step that takes it.  The last steps take the
-      // next tile's largest score.
+      // 16 score pairs, which go through three stages in three steps -- scaled; exp2; packed -- so that no stage waits
+      // for the one before; a pair is packed before the PV step that takes it.  The last steps take the next tile's
+      // largest score.  The sums of the packed pairs come after the last MFMA, in its shadow (947 us -> 916 for 4,096 on
+      // 16,384; two fewer instructions a step is what counts).
       constexpr int kQ = 2 * C::QN, kPV = 4 * C::DB, kSpread = kQ + 3 * C::DB - 2;
       constexpr int kMaxAt = kQ + 4, kMaxPer = 16 / (kPV - 4) + (16 % (kPV - 4) != 0);
       static_assert(kQ + 3 * C::DB >= kSpread + 2, "the last pairs are packed in time");
@@ -919,6 +921,8 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
       for (int i = 0; i < kQ + kPV; ++i) {
         if (i < kQ) {
           sn[i & 1] = Half<T>::mma(op[i % (kAhead + 1)], q[i >> 1], i < 2 ? f32x16{} : sn[i & 1]);
+          // (Holds the MFMA to its step: its result is wanted late, and the compiler moved half of them to the end.)
+          if (i >= 2) asm volatile("" : "+v"(sn[i & 1]));
         } else {
           const int j = i - kQ;
           o[j % C::DB] = Half<T>::mma(op[i % (kAhead + 1)], __builtin_bit_cast(QV, w[j / C::DB]), o[j % C::DB]);
@@ -927,10 +931,7 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 #pragma unroll
         for (int j = first_pair(i - 2); j < first_pair(i - 1); ++j) {
           const int nb = j >> 3, e = 2 * (j & 7);
-          const uint32_t x = pack2<T>(s[nb][e], s[nb][e + 1]);
-          w[j >> 2][j & 3] = x;
-          if (j & 1) l1 = Half<T>::sum2(x, l1);
-          else l0 = Half<T>::sum2(x, l0);
+          w[j >> 2][j & 3] = pack2<T>(s[nb][e], s[nb][e + 1]);
         }
 #pragma unroll
         for (int j = first_pair(i - 1); j < first_pair(i); ++j) {
@@ -948,6 +949,11 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) 
         for (int j = (i - kMaxAt) * kMaxPer; j < (i - kMaxAt + 1) * kMaxPer && j < 16; ++j)
           if (j >= 0) hi[j & 3] = max3(hi[j & 3], sn[j & 1][j & ~1], sn[j & 1][j | 1]);
         __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        l0 = Half<T>::sum2(w[j >> 2][j & 3], l0);
+        l1 = Half<T>::sum2(w[j >> 2][(j + 1) & 3], l1);
       }
       l += l0 + l1;
       high = fmaxf(max3(hi[0], hi[1], hi[2]), hi[3]);
