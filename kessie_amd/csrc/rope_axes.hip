@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kMaxHalf = 128;  // rotary_dim <= 256
 constexpr int kMaxAxes = 4;
+constexpr int kGridShift = 21;  // workgroups in x before y counts (a launch counts a dimension's threads in 32 bits)
 
 struct Args {
   // Rows of (token, head): x at src + t*s_ts + h*s_hs, written to dst.
@@ -153,9 +154,9 @@ __global__ __launch_bounds__(kThreads) void rope_axes_vec(Args a) {
   constexpr int N = Vec16<T>::N;
   __shared__ float2 cs[kTok * kMaxHalf];
   const int half = a.half, R = 2 * half;
-  const int64_t tile = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-  if (tile * kTok >= a.T) return;
-  const int t0 = (int)tile * kTok;
+  const uint32_t at = ((blockIdx.y << kGridShift) + blockIdx.x) * kTok;
+  if (at >= (uint32_t)a.T) return;
+  const int t0 = (int)at;
   const int ntok = min(kTok, a.T - t0);
   const int heads = kPages ? a.Hk : a.Hq + a.Hk + a.Hv;
   const int per = kPer > 0 ? kPer : a.D / (2 * N);  // steps a row
@@ -290,9 +291,8 @@ int launch(const Args& a, hipStream_t s) {
                    fine(a.ko, a.ko_ts, a.ko_hs) && fine(a.v, a.v_ts, a.v_hs) && fine(a.pool, a.tok_stride, a.head_stride) &&
                    (a.pool == nullptr || (a.page_stride % N == 0 && a.kv_stride % N == 0));
   const int heads = a.Hq + a.Hk + a.Hv;
-  // (A launch's x dimension counts its threads in 32 bits.)
   auto tiles = [&](int64_t tok) {
-    const int64_t n = div_up((int64_t)a.T, tok), x = n < 1 << 21 ? n : 1 << 21;
+    const int64_t n = div_up((int64_t)a.T, tok), x = n < 1 << kGridShift ? n : 1 << kGridShift;
     return dim3((unsigned)x, (unsigned)div_up(n, x));
   };
   if (!vec) {
