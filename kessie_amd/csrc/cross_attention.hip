@@ -533,8 +533,9 @@ __device__ __forceinline__ bool find_piece(const Args& a, int x, int rows, int k
       work += w;
     }
     if (a.B > 64) mine = lane_sequence(a, 0, lane);
-    // (ceil, and a little more for what the sums were rounded off: at most `shares` pieces and one a row tile.)
-    limit = uniform(max((int)fminf(ceilf(work / (float)a.shares * 1.0001f), 1.0e9f), a.min_steps));
+    // (ceil, and a little more for what the sums were rounded off, 2^-24 each of B / 64 + 10: at most `shares` pieces and
+    // one a row tile.)
+    limit = uniform(max((int)fminf(ceilf(work / (float)a.shares * (1.0001f + 1.0e-8f * (float)a.B)), 1.0e9f), a.min_steps));
   }
   // Long pieces (more than half the limit: all pieces of tiles that are cut are) are numbered first, so that the short
   // ones fill the end.

@@ -182,10 +182,9 @@ class KeSSieKernels:
 
     def rope_remap_axes(self, pool, page_list, orig_positions, target_positions, inv_freq, sections,
                         interleaved: bool = False, adjacent: bool = False, layout: str = "native", stream=None):
-        """Positions [axes, T]; page_list None: pool is a dense K tensor [T, H, D]."""
+        """Positions [axes, T], page_list int32; page_list None: pool is a dense K tensor [T, H, D]."""
         ops.rope_remap_axes(pool, orig_positions, target_positions, inv_freq, sections, interleaved, adjacent,
-                            page_list=None if page_list is None else page_list.to(torch.int32), layout=layout,
-                            stream=self._resolve_stream(stream))
+                            page_list=page_list, layout=layout, stream=self._resolve_stream(stream))
         self._finish(stream)
 
     def cross_attention(self, q, k, v, query_start_loc, max_query_len: int, kv_start, kv_lens, max_kv_len: int,

@@ -370,3 +370,24 @@ def test_testing_switches(dev, monkeypatch):
         attend(c, out=out)
     monkeypatch.delenv("KESSIE_REQUIRE_MFMA")
     check(c, attend(c))
+
+
+def test_many_sequences_and_a_long_one(dev):
+    """20,000 sequences of no or few states around one whose rows are cut: every piece has a workgroup."""
+    gen_ = torch.Generator().manual_seed(3)
+    seqs = [(int(c), int(n)) for c, n in zip(torch.randint(0, 3, (20000,), generator=gen_), torch.randint(0, 4, (20000,), generator=gen_))]
+    for at in (0, 12345, 19999):
+        seqs[at] = (90, 40000)
+    c = case(dev, seqs, 2, 1, 64, torch.bfloat16, seed=17)
+    got = attend(c)
+    assert torch.equal(got, attend(c))
+    starts = [sum(x for x, _ in seqs[:i]) for i in (0, 12345, 19999)]
+    for i, s in zip((0, 12345, 19999), starts):  # alone: the same rows within both roundings
+        one = {**c, "q": c["q"][s:s + 90].contiguous(), "qs": torch.tensor([0, 90], dtype=torch.int32, device=dev), "ks": c["ks"][i:i + 1].contiguous(),
+               "kl": c["kl"][i:i + 1].contiguous(), "seqs": [(90, 40000)], "starts": [c["starts"][i]]}
+        check(one, got[s:s + 90])
+    some = [i for i, (x, n) in enumerate(seqs[:300]) if x and i]
+    for i in some[:40]:
+        x, n = seqs[i]
+        s = sum(y for y, _ in seqs[:i])
+        check({**c, "q": c["q"][s:s + x].contiguous(), "seqs": [(x, n)], "starts": [c["starts"][i]]}, got[s:s + x])

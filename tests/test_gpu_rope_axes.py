@@ -256,3 +256,26 @@ def test_another_stream(dev):
     ops.rope_axes(q, None, pos, inv, (16, 24, 24), q_out=out, stream=s)
     s.synchronize()
     assert torch.equal(out, want)
+
+
+def test_kernels_class(dev):
+    from kessie_amd import ops
+    from kessie_amd.kessie_hip_ctypes import KeSSieKernels
+    k = KeSSieKernels()
+    a, b, inv = positions(dev, 3, 70, 5000, 1), positions(dev, 3, 70, 5000, 2), inv_freq(64, 1e4, dev)
+    pages = randperm(9, dev, 3)[:5].contiguous()
+    pool = randn((9, 16, 2, 2, 128), torch.bfloat16, dev, 4)
+    want, got = pool.clone(), [pool.clone(), pool.clone()]
+    ops.rope_remap_axes(want, a, b, inv, (16, 24, 24), page_list=pages)
+    k.rope_remap_axes(got[0], pages, a, b, inv, (16, 24, 24))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    k.rope_remap_axes(got[1], pages, a, b, inv, (16, 24, 24), stream=s)
+    s.synchronize()
+    assert torch.equal(got[0], want) and torch.equal(got[1], want) and not torch.equal(want, pool)
+    dense = randn((70, 2, 128), torch.bfloat16, dev, 5)
+    ref = rotate64(dense, b.long() - a, inv, (16, 24, 24))
+    k.rope_remap_axes(dense, None, a, b, inv, (16, 24, 24))
+    check(dense, ref)
+    with pytest.raises(TypeError):
+        k.rope_remap_axes(pool, pages.long(), a, b, inv, (16, 24, 24))
