@@ -761,7 +761,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 constexpr float kSlack = 8.0f;
 
 // States of a tile of cross_tile_kernel: 64 KiB of LDS or 32, so that two workgroups of four waves share a CU, and each
-// SIMD has one's softmax to run beside the other's MFMAs (fp32, head_dim 128: 2 x 1,000 on 4,000, 8 heads, 267 us against 344 with one).
+// SIMD has one's softmax to run beside the other's MFMAs (fp32, head_dim 128: 2 x 1,000 on 4,000, 8 heads, 267 us
+// against 344 with one).
 __host__ __device__ constexpr int tile_keys(int row_bytes) { return row_bytes == 512 ? 32 : 64; }
 
 // Prompts: W waves of 32 rows each over tiles of 64 states that the workgroup
@@ -1230,7 +1231,8 @@ Plan make_plan(int B, int max_q, int Tq, int Hq, int Hkv, int D, int max_kv, int
   // states of 32 rows and merge them in LDS.  1 x 60 on 600 (bf16, 8 heads of 128) 12.3 us against 15.3 with 128 rows a
   // workgroup, 1 x 300 on 100 (fp32, 8 heads of 128) 16.9 against 22.9; past that it loses: 1 x 60 on 1,000 15.7 against
   // 13.6, 2 x 60 on 180 in fp32 21.5 against 13.9, 4 x 50..101 on 577 (fp32, 12 heads of 64) 21.7 against 20.0.
-  const bool small = tiles_of(32) * Hkv <= (int64_t)cus * rows_per_cu && max_kv <= (es == 2 ? 5 : row_bytes == 512 ? 2 : 3) * nw * kRowsKeys;
+  const int small_kv = (es == 2 ? 5 : row_bytes == 512 ? 2 : 3) * nw * kRowsKeys;
+  const bool small = tiles_of(32) * Hkv <= (int64_t)cus * rows_per_cu && max_kv <= small_kv;
   if (most <= 32 || small) {
     p.tiles = most <= 32 ? B : tiles_of(32);
     p.part_rows = (int)(most < 32 ? most : 32);
